@@ -215,6 +215,83 @@ int nb_rnn_plan_create(nb_handle_t handle, const nb_rnn_desc_t *desc, nb_plan_t 
 int nb_rnn_set_weights(nb_plan_t plan, const float *blob_stream, size_t count, int mem);
 int nb_rnn_forward(nb_plan_t plan, const float *x, float *out);
 
+/* --------------------------------------------------------- linear attention */
+/* Linear attention with a decay for each head: the recurrent layer of language models whose state does not grow with
+ * the sequence (no counterpart in the reference, whose recurrent layers are lstm_layer.cc and rnn_layer.cc).  Per
+ * sequence and head a state S [key_dim][value_dim] in fp32, and over its tokens
+ *     S_t = exp(g_t) S_{t-1} + k_t v_t^T        out_t = scale * q_t^T S_t
+ * Log decays g are fp32, usually <= 0; -inf forgets everything before the token.  Head h reads query and key head
+ * h / (heads / key_heads).  q, k, v and out have the plan's type; the state is always fp32, and so is everything between
+ * the inputs and the one rounding of out.  fp32 tensors are multiplied with fp32-level agreement in every math mode. */
+typedef enum { NB_DTYPE_F32 = 0, NB_DTYPE_BF16 = 1 } nb_dtype;
+typedef struct {
+    int batch, time_steps;                  /* sequences, and tokens of the longest */
+    int heads, key_heads;                   /* of v and out, of q and k */
+    int key_dim, value_dim;                 /* of a head: 1 to 256 */
+    int dtype;                              /* nb_dtype of q, k, v, out */
+    float scale;
+} nb_linear_attention_desc_t;
+/* Element (b, t, head, i) is data[b*batch_stride + t*token_stride + head*head_stride + i], strides in elements and not
+ * negative; inputs may repeat values with strides of 0 (a decay per head: batch_stride = token_stride = 0).  Packed
+ * sequences: batch_stride is not read, t counts all tokens. */
+typedef struct {
+    void *data;
+    long long batch_stride, token_stride, head_stride;
+} nb_tokens_t;
+/* Device pointers.
+ *   log_decay: fp32, one value a head (i = 0); data NULL: no decay.
+ *   offsets [batch+1]: sequence b is tokens offsets[b] to offsets[b+1]-1 of tensors of `tokens` tokens.  NULL: sequence b is
+ *     at b*batch_stride, with lengths[b] tokens, or time_steps where lengths is NULL too.  Rows of out that belong to no
+ *     sequence are not written; tokens past time_steps are not read.  A sequence may be empty: its state passes through.
+ *   state [state_slots][heads][key_dim][value_dim]: S before the first token, NULL: zeros.  state_out: S after the last
+ *     token, NULL: not wanted (a step then writes to state); it may be state itself.  Only slots in use are written.
+ *   slots [batch]: the slot of each sequence's state, all different; NULL: slot b.  A sequence whose slot is not in
+ *     [0, state_slots) is not served: its rows of out are zeros, and it has no state. */
+typedef struct {
+    nb_tokens_t q, k, v, log_decay, out;
+    const int *offsets, *lengths;
+    long long tokens;
+    const float *state;
+    float *state_out;
+    const int *slots;
+    long long state_slots;                  /* 0: batch */
+} nb_linear_attention_io_t;
+int nb_linear_attention_plan_create(nb_handle_t handle, const nb_linear_attention_desc_t *desc, nb_plan_t *plan);
+/* Prompts, in chunks of tokens: any number of tokens per sequence. */
+int nb_linear_attention_forward(nb_plan_t plan, const nb_linear_attention_io_t *io);
+/* One token of every sequence (token strides are not read; no offsets or lengths); state is required. */
+int nb_linear_attention_step(nb_plan_t plan, const nb_linear_attention_io_t *io);
+
+/* Norms before and after a block, with its gate, its residual scale and the residual sum (no counterpart in the
+ * reference).  Per row of `width` values:
+ *     n = norm(x) * weight + bias             over each of `groups` groups of the row (the heads behind an attention)
+ *     s = residual + scale * channel_scale * (n * gate_function(gate))       -> sum, may be NULL if y is not
+ *     y = next_norm(s) * next_weight + next_bias      over the whole row: the norm in front of the next block
+ * Every pointer but x may be NULL for "not there".  Weights [width] are fp32.  s keeps its 32 bits up to the second norm.
+ * sum may be residual, and y may be x.  Rows have up to 32768 values. */
+typedef enum { NB_NORM_NONE = 0, NB_NORM_RMS = 1, NB_NORM_LAYER = 2 } nb_norm;
+typedef enum { NB_GATE_NONE = 0, NB_GATE_LINEAR = 1, NB_GATE_SIGMOID = 2, NB_GATE_SILU = 3 } nb_gate;
+typedef struct {
+    int rows, width, groups;
+    int norm, next_norm;                    /* nb_norm */
+    int gate;                               /* nb_gate */
+    int dtype;                              /* nb_dtype of x, gate, y */
+    int residual_dtype;                     /* nb_dtype of residual, sum: dtype, or fp32 */
+    float eps, scale;
+    long long x_stride, gate_stride, residual_stride, sum_stride, y_stride;     /* of rows, in elements; 0: width */
+} nb_norm_gate_desc_t;
+typedef struct {
+    const void *x;
+    const float *weight, *bias;
+    const void *gate;
+    const float *channel_scale;
+    const void *residual;
+    void *sum;
+    const float *next_weight, *next_bias;
+    void *y;
+} nb_norm_gate_io_t;
+int nb_norm_gate_residual(nb_handle_t handle, const nb_norm_gate_desc_t *desc, const nb_norm_gate_io_t *io);
+
 /* ------------------------------------------------------- operator library */
 /* _<name>_activation_(out, n) (common/activations.h:38-50), in place. */
 int nb_activation_forward(nb_handle_t handle, int activation, float *data, size_t n);

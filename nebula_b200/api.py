@@ -9,6 +9,7 @@ raise.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -21,6 +22,9 @@ MATH_MODES = {"tf32": MATH_TF32, "tf32x3": MATH_TF32X3, "fp32": MATH_FP32}
 LAYOUT_NCHW, LAYOUT_NHWC = 0, 1
 POOL_MAX, POOL_AVG = 0, 1
 MEM_HOST, MEM_DEVICE = 0, 1
+DTYPES = {"f32": 0, "bf16": 1}
+NORMS = {"none": 0, "rms": 1, "layer": 2}
+GATES = {"none": 0, "linear": 1, "sigmoid": 2, "silu": 3}
 ACT = {"elu": 1, "hardtan": 2, "leaky": 3, "lhtan": 4, "linear": 5, "loggy": 6, "logistic": 7, "plse": 8,
        "ramp": 9, "relie": 10, "relu": 11, "stair": 12, "tanh": 13}
 STATUS = {0: "NB_OK", 1: "NB_ERR_INVALID_ARG", 2: "NB_ERR_CUDA", 3: "NB_ERR_UNSUPPORTED", 4: "NB_ERR_WEIGHTS",
@@ -55,6 +59,16 @@ class LstmDesc(C.Structure):
 
 class RnnDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("time_steps", "batch", "inputs", "hidden", "batch_normalize", "activation")]
+
+
+class LinearAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("batch", "time_steps", "heads", "key_heads", "key_dim", "value_dim", "dtype")] + [("scale", C.c_float)]
+
+
+# nb_linear_attention_io_t and nb_norm_gate_desc_t / nb_norm_gate_io_t: filled by one pack_into per call
+_ATTENTION_IO = struct.Struct("=27q")
+_NORM_DESC = struct.Struct("=8i2f5q")
+_NORM_IO = struct.Struct("=10q")
 
 
 class ConvFusion(C.Structure):
@@ -114,6 +128,10 @@ SIGNATURES = {
     "nb_rnn_plan_create": (C.c_int, [_VP, C.POINTER(RnnDesc), C.POINTER(_VP)]),
     "nb_rnn_set_weights": (C.c_int, [_VP, _VP, C.c_size_t, C.c_int]),
     "nb_rnn_forward": (C.c_int, [_VP, _VP, _VP]),
+    "nb_linear_attention_plan_create": (C.c_int, [_VP, C.POINTER(LinearAttentionDesc), C.POINTER(_VP)]),
+    "nb_linear_attention_forward": (C.c_int, [_VP, _VP]),
+    "nb_linear_attention_step": (C.c_int, [_VP, _VP]),
+    "nb_norm_gate_residual": (C.c_int, [_VP, _VP, _VP]),
     "nb_activation_forward": (C.c_int, [_VP, C.c_int, _VP, C.c_size_t]),
     "nb_forward_bias": (C.c_int, [_VP, _VP, _VP, C.c_uint, C.c_uint, C.c_uint]),
     "nb_batchnorm_normalize": (C.c_int, [_VP, _VP, _VP, _VP, C.c_uint, C.c_uint, C.c_uint]),
@@ -292,6 +310,53 @@ class Handle:
         self.check(self.lib.nb_softmax_forward(self.h, _ptr(x), _ptr(y), rows, classes))
         return y
 
+    def norm_gate_residual(self, x, weight=None, bias=None, norm="rms", groups=1, eps=1e-6, gate=None, gate_act="silu", residual=None,
+                           scale=1.0, channel_scale=None, next_norm="none", next_weight=None, next_bias=None, out=None, y=None):
+        """s = residual + scale * channel_scale * (norm(x) * gate function(gate)) and y = next_norm(s), row by row
+        (nb_norm_gate_residual); x [..., width], float32 or bfloat16, rows evenly spaced.  Returns (s, y), y None without a second
+        norm.  `out` may be the residual itself."""
+        import torch
+        width = x.shape[-1]
+        kinds = {torch.float32: 0, torch.bfloat16: 1}
+        kind = kinds.get(x.dtype)
+        if kind is None or not x.is_cuda:
+            raise NebulaError(1, "norm: x is a float32 or bfloat16 tensor on the device")
+        if out is None:
+            out = torch.empty(x.shape, device=x.device, dtype=x.dtype if residual is None else residual.dtype)
+        if y is None and next_norm != "none":
+            y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        rows = x.numel() // width if width else 0
+        a = [0] * 5
+        s = [0] * 5
+        for i, t in enumerate((x, gate, residual, out, y)):
+            if t is None:
+                continue
+            if t.shape != x.shape or t.device != x.device:
+                raise NebulaError(1, "norm: tensors of different shapes or devices")
+            if i in (1, 4) and t.dtype != x.dtype or i == 3 and residual is not None and t.dtype != residual.dtype:
+                raise NebulaError(1, "norm: gate and y have the type of x, the sum that of the residual")
+            if t.is_contiguous():
+                s[i] = width
+            elif t.dim() == 2 and t.stride(1) == 1:
+                s[i] = t.stride(0)
+            else:
+                raise NebulaError(1, "norm: rows are contiguous, and evenly spaced in two dimensions")
+            a[i] = t.data_ptr()
+        w = [0] * 5
+        for i, t in enumerate((weight, bias, channel_scale, next_weight, next_bias)):
+            if t is None:
+                continue
+            if t.dtype != torch.float32 or t.numel() != width or not t.is_contiguous() or t.device != x.device:
+                raise NebulaError(1, "norm: weights are contiguous float32 tensors of the row's width")
+            w[i] = t.data_ptr()
+        rkind = kinds.get(out.dtype, -1)
+        desc, io = bytearray(_NORM_DESC.size), bytearray(_NORM_IO.size)
+        _NORM_DESC.pack_into(desc, 0, rows, width, groups, NORMS[norm], NORMS[next_norm], GATES[gate_act] if gate is not None else 0, kind,
+                             rkind, eps, scale, *s)
+        _NORM_IO.pack_into(io, 0, a[0], w[0], w[1], a[1], w[2], a[2], a[3], w[3], w[4], a[4])
+        self.check(self.lib.nb_norm_gate_residual(self.h, (C.c_char * len(desc)).from_buffer(desc), (C.c_char * len(io)).from_buffer(io)))
+        return out, y
+
     def gemm(self, ta, tb, M, N, K, alpha, A, lda, B, ldb, beta, Cm, ldc):
         self.check(self.lib.nb_gemm(self.h, int(ta), int(tb), M, N, K, alpha, _ptr(A), lda, _ptr(B), ldb, beta,
                                     _ptr(Cm), ldc))
@@ -428,6 +493,91 @@ class Rnn(_Plan):
         out = torch.empty((d.time_steps, d.batch, d.hidden), device=x.device, dtype=torch.float32)
         self.handle.check(self.handle.lib.nb_rnn_forward(self.p, _ptr(x), _ptr(out)))
         return out
+
+
+class LinearAttention(_Plan):
+    """Linear attention with a decay for each head (nb_linear_attention_*): forward() over prompts, step() for one token of
+    every sequence.  No weights: queries, keys, values and log decays come from the layers around it.
+
+    Tensors are float32 or bfloat16 ("f32" / "bf16") with contiguous head vectors and any strides otherwise: q, k
+    [batch, tokens, key_heads, key_dim], v and the result [batch, tokens, heads, value_dim]; packed sequences (`offsets`, int32
+    [batch + 1]) and steps have one leading dimension.  log_decay is float32: [..., heads] like v without its last dimension, or
+    [heads]; None: no decay.  The state pool is a contiguous float32 tensor [slots, heads, key_dim, value_dim]."""
+
+    def __init__(self, handle, batch, time_steps, heads, key_dim, value_dim, key_heads=None, dtype="bf16", scale=1.0):
+        import torch
+        super().__init__(handle)
+        self.desc = LinearAttentionDesc(batch, time_steps, heads, key_heads or heads, key_dim, value_dim, DTYPES[dtype], scale)
+        handle.check(handle.lib.nb_linear_attention_plan_create(handle.h, C.byref(self.desc), C.byref(self.p)))
+        self.dtype = torch.float32 if dtype == "f32" else torch.bfloat16
+        self._key, self._value = (self.desc.key_heads, key_dim), (heads, value_dim)
+        self._state = (heads, key_dim, value_dim)
+        self._io = (C.c_char * _ATTENTION_IO.size)()
+
+    def _view(self, t, lead, tail, what):
+        """Address and strides (batch, token, head) of a tensor of tokens."""
+        if t.dtype != self.dtype or t.shape[:-2] != lead or tuple(t.shape[-2:]) != tail or (tail[1] > 1 and t.stride(-1) != 1) or not t.is_cuda:
+            raise NebulaError(1, f"linear attention: {what} is {tuple(t.shape)} {t.dtype} with last stride {t.stride(-1)}, expected "
+                                 f"{(*lead, *tail)} {self.dtype} on the device with contiguous head vectors")
+        st = t.stride()
+        if len(lead) == 2:
+            return t.data_ptr(), st[0], st[1], st[2]
+        return t.data_ptr(), st[0], st[0], st[1]
+
+    def _decay(self, g, lead):
+        if g is None:
+            return 0, 0, 0, 0
+        if str(g.dtype) != "torch.float32" or not g.is_cuda or g.shape[-1] != self._value[0] or (g.dim() > 1 and g.shape[:-1] != lead):
+            raise NebulaError(1, f"linear attention: log_decay is {tuple(g.shape)} {g.dtype}, expected float32 {(*lead, self._value[0])} or "
+                                 f"{(self._value[0],)} on the device")
+        st = g.stride()
+        if g.dim() == 1:
+            return g.data_ptr(), 0, 0, st[0]
+        if len(lead) == 2:
+            return g.data_ptr(), st[0], st[1], st[2]
+        return g.data_ptr(), st[0], st[0], st[1]
+
+    def _ints(self, t, n, what):
+        if t is None:
+            return 0
+        if str(t.dtype) != "torch.int32" or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
+            raise NebulaError(1, f"linear attention: {what} is a contiguous int32 tensor of {n} values on the device")
+        return t.data_ptr()
+
+    def _pool(self, t, slots, what):
+        if t is None:
+            return 0
+        if str(t.dtype) != "torch.float32" or tuple(t.shape[1:]) != self._state or t.shape[0] != slots or not t.is_contiguous() or not t.is_cuda:
+            raise NebulaError(1, f"linear attention: {what} is a contiguous float32 tensor {(slots, *self._state)} on the device")
+        return t.data_ptr()
+
+    def _run(self, fn, lead, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out):
+        import torch
+        if out is None:
+            out = torch.empty((*lead, *self._value), device=v.device, dtype=self.dtype)
+        batch = self.desc.batch
+        pool = state if state is not None else state_out
+        n = pool.shape[0] if pool is not None and slots is not None else batch
+        _ATTENTION_IO.pack_into(
+            self._io, 0, *self._view(q, lead, self._key, "q"), *self._view(k, lead, self._key, "k"), *self._view(v, lead, self._value, "v"),
+            *self._decay(log_decay, lead), *self._view(out, lead, self._value, "out"), self._ints(offsets, batch + 1, "offsets"),
+            self._ints(lengths, batch, "lengths"), lead[0] if offsets is not None else 0, self._pool(state, n, "state"),
+            self._pool(state_out, n, "state_out"), self._ints(slots, batch, "slots"), n)
+        self.handle.check(fn(self.p, self._io))
+        return out
+
+    def forward(self, q, k, v, log_decay=None, state=None, state_out=None, offsets=None, lengths=None, slots=None, out=None):
+        """Prompts.  `state` is read before the first token of a sequence (None: zeros), `state_out` written behind the last
+        (None: not kept; it may be `state`)."""
+        lead = v.shape[:-2] if offsets is not None else (self.desc.batch, self.desc.time_steps)
+        if len(lead) != (1 if offsets is not None else 2):
+            raise NebulaError(1, "linear attention: packed tensors are [tokens, heads, size]")
+        return self._run(self.handle.lib.nb_linear_attention_forward, lead, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out)
+
+    def step(self, q, k, v, log_decay=None, state=None, state_out=None, slots=None, out=None):
+        """One token of every sequence, tensors [batch, heads, size]; updates `state`, or writes the new one to `state_out`."""
+        return self._run(self.handle.lib.nb_linear_attention_step, (self.desc.batch,), q, k, v, log_decay, state, state_out, None, None,
+                         slots, out)
 
 
 class Network:

@@ -6,6 +6,7 @@
 #include <cstring>
 #include <fstream>
 
+#include "linear_attention.h"
 #include "network.h"
 
 using namespace nb;
@@ -281,6 +282,7 @@ int nb_plan_prepare(nb_plan_t plan) {
             }
             case NB_PLAN_LSTM: static_cast<LstmPlan *>(plan)->reserve(true, false, false); break;
             case NB_PLAN_RNN: static_cast<RnnPlan *>(plan)->reserve(false); break;
+            case NB_PLAN_LINEAR_ATTENTION: static_cast<LinAttnPlan *>(plan)->reserve(); break;
             default: throw Error(NB_ERR_INVALID_ARG, "unknown plan kind");
         }
         NB_CHECK_CUDA(cudaStreamSynchronize(plan->h->stream));
@@ -385,7 +387,43 @@ int nb_rnn_forward(nb_plan_t plan, const float *x, float *out) {
     });
 }
 
+int nb_linear_attention_plan_create(nb_handle_t h, const nb_linear_attention_desc_t *desc, nb_plan_t *plan) {
+    if (!h || !plan) return NB_ERR_INVALID_ARG;
+    *plan = nullptr;
+    return guarded(h, [&] {
+        NB_REQUIRE(desc != nullptr, "null descriptor");
+        DeviceGuard g(h->device);
+        *plan = new LinAttnPlan(h, *desc);
+    });
+}
+int nb_linear_attention_forward(nb_plan_t plan, const nb_linear_attention_io_t *io) {
+    if (!plan) return NB_ERR_INVALID_ARG;
+    return guarded(plan->h, [&] {
+        NB_REQUIRE(plan->kind == NB_PLAN_LINEAR_ATTENTION, "not a linear-attention plan");
+        NB_REQUIRE(io != nullptr, "null argument");
+        DeviceGuard g(plan->h->device);
+        static_cast<LinAttnPlan *>(plan)->forward(*io);
+    });
+}
+int nb_linear_attention_step(nb_plan_t plan, const nb_linear_attention_io_t *io) {
+    if (!plan) return NB_ERR_INVALID_ARG;
+    return guarded(plan->h, [&] {
+        NB_REQUIRE(plan->kind == NB_PLAN_LINEAR_ATTENTION, "not a linear-attention plan");
+        NB_REQUIRE(io != nullptr, "null argument");
+        DeviceGuard g(plan->h->device);
+        static_cast<LinAttnPlan *>(plan)->step(*io);
+    });
+}
+
 // ------------------------------------------------------- stateless operators
+int nb_norm_gate_residual(nb_handle_t h, const nb_norm_gate_desc_t *d, const nb_norm_gate_io_t *io) {
+    if (!h) return NB_ERR_INVALID_ARG;
+    return guarded(h, [&] {
+        NB_REQUIRE(d && io, "null argument");
+        DeviceGuard g(h->device);
+        launch_norm_gate(h, *d, *io);
+    });
+}
 int nb_pool_forward(nb_handle_t h, const nb_pool_desc_t *d, const float *x, float *y) {
     if (!h) return NB_ERR_INVALID_ARG;
     return guarded(h, [&] {

@@ -1,0 +1,274 @@
+// Linear attention with a decay for each head (no counterpart in the reference, whose recurrent layers are LSTM and RNN,
+// lstm_layer.cc:233-346): a state S [key_dim][value_dim] per sequence and head,
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t,
+// over the tokens of a prompt, and for one token of every sequence of a batch.
+#include "linear_attention.h"
+
+#include "device_math.cuh"
+
+namespace nb {
+
+namespace {
+
+constexpr int MAX_DIM = 256;
+
+// ------------------------------------------------------------------ single tokens
+// S' = exp(g) S + k v^T and o = scale q^T S'.  Bound by the state, which is read and written once: 8 bytes a value for 5
+// operations.  A CTA takes `cols` columns of one sequence and head: a thread owns one quad (V = 1: one value) of columns of the
+// rows that are congruent to its own, so that a warp's accesses are whole lines, and keeps its part of q^T S' for the columns in
+// registers; the parts are added in the order of the rows.
+// The decay is applied as S + expm1(g) S.  exp(g) rounded to fp32 is off by up to 2^-25, the same way at every token of a head with a
+// fixed decay: over a memory of thousands of tokens that adds up to thousands of roundings (a state of 32768 tokens was 3e-4
+// off), while expm1(g) is off by a share of itself.  A decay of zero (expm1 = -1) forgets whatever was there, infinities and NaN too.
+constexpr int STEP_TPB = 256;
+template <class T, int V>
+__global__ void __launch_bounds__(STEP_TPB) linear_attention_step_kernel(LinAttnParams p, int cols, int tiles) {
+    grid_begin();
+    __shared__ float qs[MAX_DIM], ks[MAX_DIM];
+    __shared__ float part[STEP_TPB * V];
+    const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % p.H, b = bh / p.H;
+    const int width = cols / V, lanes = STEP_TPB / width;       // threads along a row, rows at a time
+    const int c = threadIdx.x % width, r0 = threadIdx.x / width, col = tile * cols + c * V;
+    const SeqAt s = seq_at(p, b);
+    T *out = (T *)p.out.p + b * p.out.batch + h * p.out.head;
+    if (s.slot < 0) {
+        for (int i = threadIdx.x; i < cols && tile * cols + i < p.dv; i += STEP_TPB) out[tile * cols + i] = from_f32<T>(0.0f);
+        return;
+    }
+    const T *q = (const T *)p.q.p + b * p.q.batch + h / p.group * p.q.head;
+    const T *k = (const T *)p.k.p + b * p.k.batch + h / p.group * p.k.head;
+    const T *v = (const T *)p.v.p + b * p.v.batch + h * p.v.head;
+    for (int i = threadIdx.x; i < p.dk; i += STEP_TPB) {
+        qs[i] = to_f32(q[i]) * p.scale;
+        ks[i] = to_f32(k[i]);
+    }
+    const float less = p.g.p ? expm1f(((const float *)p.g.p)[b * p.g.batch + h * p.g.head]) : 0.0f;
+    const bool mine = r0 < lanes && col < p.dv;
+    float vv[V], o[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        vv[j] = mine ? to_f32(v[col + j]) : 0.0f;
+        o[j] = 0.0f;
+    }
+    __syncthreads();
+    if (mine) {
+        const long long at = (s.slot * p.H + h) * (long long)p.dk * p.dv + col;
+        const float *S = p.state + at;
+        float *So = p.state_out + at;
+        constexpr int U = 8;                // rows in flight
+        for (int r = r0; r < p.dk; r += U * lanes) {
+            float x[U][V];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int row = r + u * lanes;
+                if (row < p.dk) {
+                    if constexpr (V == 4) {
+                        const float4 f = *(const float4 *)(S + (long long)row * p.dv);
+                        x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
+                    } else {
+                        x[u][0] = S[(long long)row * p.dv];
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int row = r + u * lanes;
+                if (row < p.dk) {
+                    const float kk = ks[row], qq = qs[row];
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        x[u][j] = fmaf(kk, vv[j], less == -1.0f ? 0.0f : fmaf(less, x[u][j], x[u][j]));
+                        o[j] = fmaf(qq, x[u][j], o[j]);
+                    }
+                    if constexpr (V == 4) *(float4 *)(So + (long long)row * p.dv) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+                    else So[(long long)row * p.dv] = x[u][0];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) part[j * STEP_TPB + threadIdx.x] = o[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < cols && tile * cols + i < p.dv; i += STEP_TPB) {
+        float sum = 0.0f;
+        for (int r = 0; r < lanes; r++) sum += part[(i % V) * STEP_TPB + r * width + i / V];
+        out[tile * cols + i] = from_f32<T>(sum);
+    }
+}
+
+// ------------------------------------------------- prompts, token by token
+// The recurrence as it is written, for any sizes: a CTA takes 32 columns of one sequence and head with the state in registers,
+// its four warps a quarter of the rows each (KR per thread, rows past key_dim are zeros).  Blocks of 16 tokens are staged in
+// shared memory; queries and keys are read from there as broadcasts.  Bound by the chain of tokens.
+constexpr int REC_TPB = 128, REC_TOK = 16, REC_COLS = 32;
+template <class T, int KR>
+__global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(LinAttnParams p, int tiles) {
+    grid_begin();
+    __shared__ __align__(16) float qs[REC_TOK][4 * KR], ks[REC_TOK][4 * KR];
+    __shared__ float vs[REC_TOK][REC_COLS], part[4][REC_TOK][REC_COLS], ds[REC_TOK];
+    const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % p.H, b = bh / p.H;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = tile * REC_COLS + lane;
+    const SeqAt s = seq_at(p, b);
+    const T *q = (const T *)p.q.p + token_base(p, p.q, b, s, h / p.group), *k = (const T *)p.k.p + token_base(p, p.k, b, s, h / p.group);
+    const T *v = (const T *)p.v.p + token_base(p, p.v, b, s, h);
+    const float *g = p.g.p ? (const float *)p.g.p + token_base(p, p.g, b, s, h) : nullptr;
+    T *out = (T *)p.out.p + token_base(p, p.out, b, s, h);
+    if (s.slot < 0) {
+        for (int t = warp; t < s.len; t += 4)
+            if (col < p.dv) out[t * p.out.token + col] = from_f32<T>(0.0f);
+        return;
+    }
+    const long long at = (s.slot * p.H + h) * (long long)p.dk * p.dv + col;
+    float S[KR];
+#pragma unroll
+    for (int i = 0; i < KR; i++) {
+        const int row = warp * KR + i;
+        S[i] = p.state && row < p.dk && col < p.dv ? p.state[at + (long long)row * p.dv] : 0.0f;
+    }
+    for (int t0 = 0; t0 < s.len; t0 += REC_TOK) {
+        const int n = min(REC_TOK, s.len - t0);
+        for (int i = threadIdx.x; i < REC_TOK * 4 * KR; i += REC_TPB) {
+            const int t = i / (4 * KR), d = i % (4 * KR);
+            const bool in = t < n && d < p.dk;
+            qs[t][d] = in ? to_f32(q[(t0 + t) * p.q.token + d]) : 0.0f;
+            ks[t][d] = in ? to_f32(k[(t0 + t) * p.k.token + d]) : 0.0f;
+        }
+        for (int t = warp; t < REC_TOK; t += 4) vs[t][lane] = t < n && col < p.dv ? to_f32(v[(t0 + t) * p.v.token + col]) : 0.0f;
+        if (threadIdx.x < REC_TOK) ds[threadIdx.x] = threadIdx.x < n && g ? expm1f(g[(t0 + threadIdx.x) * p.g.token]) : 0.0f;
+        __syncthreads();
+        for (int t = 0; t < n; t++) {
+            const float d = ds[t], vv = vs[t][lane];
+            float o0 = 0.0f, o1 = 0.0f, o2 = 0.0f, o3 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KR; i += 4) {
+                const float4 kk = *(const float4 *)&ks[t][warp * KR + i], qq = *(const float4 *)&qs[t][warp * KR + i];
+                S[i] = fmaf(kk.x, vv, d == -1.0f ? 0.0f : fmaf(d, S[i], S[i]));
+                S[i + 1] = fmaf(kk.y, vv, d == -1.0f ? 0.0f : fmaf(d, S[i + 1], S[i + 1]));
+                S[i + 2] = fmaf(kk.z, vv, d == -1.0f ? 0.0f : fmaf(d, S[i + 2], S[i + 2]));
+                S[i + 3] = fmaf(kk.w, vv, d == -1.0f ? 0.0f : fmaf(d, S[i + 3], S[i + 3]));
+                o0 = fmaf(qq.x, S[i], o0);
+                o1 = fmaf(qq.y, S[i + 1], o1);
+                o2 = fmaf(qq.z, S[i + 2], o2);
+                o3 = fmaf(qq.w, S[i + 3], o3);
+            }
+            part[warp][t][lane] = (o0 + o1) + (o2 + o3);
+        }
+        __syncthreads();
+        for (int t = warp; t < n; t += 4)
+            if (col < p.dv)
+                out[(t0 + t) * p.out.token + col] =
+                    from_f32<T>(p.scale * ((part[0][t][lane] + part[1][t][lane]) + (part[2][t][lane] + part[3][t][lane])));
+        // (the next block's staging touches nothing that this reads, and is followed by a barrier before `part` is written)
+    }
+    if (p.state_out)
+#pragma unroll
+        for (int i = 0; i < KR; i++) {
+            const int row = warp * KR + i;
+            if (row < p.dk && col < p.dv) p.state_out[at + (long long)row * p.dv] = S[i];
+        }
+}
+
+template <class T>
+void launch_recurrent(nb_handle_s *h, const LinAttnParams &p) {
+    const int tiles = (p.dv + REC_COLS - 1) / REC_COLS;
+    const dim3 grid((unsigned)(p.B * p.H * tiles));
+    if (p.dk <= 16) launch_overlapped(h, linear_attention_recurrent_kernel<T, 4>, grid, REC_TPB, 0, p, tiles);
+    else if (p.dk <= 32) launch_overlapped(h, linear_attention_recurrent_kernel<T, 8>, grid, REC_TPB, 0, p, tiles);
+    else if (p.dk <= 64) launch_overlapped(h, linear_attention_recurrent_kernel<T, 16>, grid, REC_TPB, 0, p, tiles);
+    else if (p.dk <= 128) launch_overlapped(h, linear_attention_recurrent_kernel<T, 32>, grid, REC_TPB, 0, p, tiles);
+    else launch_overlapped(h, linear_attention_recurrent_kernel<T, 64>, grid, REC_TPB, 0, p, tiles);
+    check_launch("linear_attention_recurrent_kernel");
+    count_launch(h);
+}
+
+template <class T>
+void launch_step(nb_handle_s *h, const LinAttnParams &p) {
+    const bool quads = p.dv % 4 == 0 && ((uintptr_t)p.state | (uintptr_t)p.state_out) % 16 == 0;
+    // whole rows of the state where there are CTAs enough for two per SM; fewer columns, down to 16, where there are not
+    int cols = quads ? 16 : 32;
+    while (cols < p.dv && cols < (quads ? 128 : 256)) cols *= 2;
+    while (cols > 16 && (long long)p.B * p.H * ((p.dv + cols - 1) / cols) < 2 * h->sm_count) cols /= 2;
+    const int tiles = (p.dv + cols - 1) / cols;
+    const dim3 grid((unsigned)(p.B * p.H * tiles));
+    if (quads) launch_overlapped(h, linear_attention_step_kernel<T, 4>, grid, STEP_TPB, 0, p, cols, tiles);
+    else launch_overlapped(h, linear_attention_step_kernel<T, 1>, grid, STEP_TPB, 0, p, cols, tiles);
+    check_launch("linear_attention_step_kernel");
+    count_launch(h);
+}
+
+}  // namespace
+
+LinAttnPlan::LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc) : nb_plan_s(NB_PLAN_LINEAR_ATTENTION, h), d(desc) {
+    NB_REQUIRE(d.batch > 0 && d.time_steps > 0 && d.heads > 0 && d.key_heads > 0, "linear attention: non-positive extent");
+    NB_REQUIRE(d.key_dim > 0 && d.value_dim > 0, "linear attention: non-positive head size");
+    NB_REQUIRE(d.heads % d.key_heads == 0, "linear attention: heads is not a multiple of key_heads");
+    NB_REQUIRE(d.dtype == NB_DTYPE_F32 || d.dtype == NB_DTYPE_BF16, "linear attention: unknown type");
+    if (d.key_dim > MAX_DIM || d.value_dim > MAX_DIM) throw Error(NB_ERR_UNSUPPORTED, "linear attention: heads of more than 256 values");
+    // grids are indexed in 31 bits, the smallest column tile being 16 wide
+    NB_REQUIRE((long long)d.batch * d.heads * ((d.value_dim + 15) / 16) < (1LL << 31), "linear attention: too many sequences and heads");
+}
+
+LinAttnParams LinAttnPlan::params(const nb_linear_attention_io_t &io, bool step) const {
+    const size_t size = d.dtype == NB_DTYPE_BF16 ? 2 : 4;
+    const bool packed = io.offsets != nullptr;
+    NB_REQUIRE((packed && io.tokens == 0) || (io.q.data && io.k.data && io.v.data && io.out.data), "linear attention: null tensor");
+    NB_REQUIRE(!io.out.data || (io.out.data != io.q.data && io.out.data != io.k.data && io.out.data != io.v.data), "linear attention: out is one of the inputs");
+    NB_REQUIRE(!(io.offsets && io.lengths), "linear attention: offsets (packed sequences) or lengths (padded ones), not both");
+    NB_REQUIRE(!step || (!io.offsets && !io.lengths), "linear attention: a step has one token of every sequence, without offsets or lengths");
+    NB_REQUIRE(!packed || io.tokens >= 0, "linear attention: negative number of packed tokens");
+    NB_REQUIRE(!step || io.state, "linear attention: a step needs a state");
+    NB_REQUIRE(!io.slots || io.state || io.state_out, "linear attention: slots without a state");
+    const long long slots = io.slots ? io.state_slots : d.batch;
+    NB_REQUIRE(slots > 0, "linear attention: a state pool without slots");
+    NB_REQUIRE(io.state_slots == 0 || io.state_slots >= slots, "linear attention: fewer states than sequences");
+    auto view = [&](const nb_tokens_t &t, int heads, int dim, size_t bytes, const char *what) {
+        NB_REQUIRE(t.batch_stride >= 0 && t.token_stride >= 0 && t.head_stride >= 0, std::string("linear attention: negative stride of ") + what);
+        NB_REQUIRE((uintptr_t)t.data % bytes == 0, std::string("linear attention: misaligned ") + what);
+        const long long rows = packed ? io.tokens : step ? 1 : d.time_steps;
+        if (rows > 0) {
+            const long long last = (packed ? 0 : (d.batch - 1) * t.batch_stride) + (rows - 1) * t.token_stride + (heads - 1) * t.head_stride + dim;
+            check_extent(h, t.data, 0, last * (long long)bytes, what);
+        }
+        return TokenView{t.data, t.batch_stride, t.token_stride, t.head_stride};
+    };
+    LinAttnParams p = {};
+    p.q = view(io.q, d.key_heads, d.key_dim, size, "queries");
+    p.k = view(io.k, d.key_heads, d.key_dim, size, "keys");
+    p.v = view(io.v, d.heads, d.value_dim, size, "values");
+    if (io.log_decay.data) p.g = view(io.log_decay, d.heads, 1, 4, "log decays");
+    p.out = view(io.out, d.heads, d.value_dim, size, "out");
+    // rows of out that are written must not share memory
+    NB_REQUIRE(d.heads == 1 || p.out.head >= d.value_dim, "linear attention: heads of out overlap");
+    NB_REQUIRE(step || d.time_steps == 1 || p.out.token >= d.value_dim, "linear attention: tokens of out overlap");
+    NB_REQUIRE(packed || d.batch == 1 || p.out.batch >= d.value_dim, "linear attention: sequences of out overlap");
+    p.offsets = io.offsets;
+    p.lengths = io.lengths;
+    p.slots = io.slots;
+    p.tokens = io.tokens;
+    p.state = io.state;
+    p.state_out = io.state_out ? io.state_out : step ? const_cast<float *>(io.state) : nullptr;
+    p.state_slots = slots;
+    const long long state_bytes = slots * d.heads * d.key_dim * d.value_dim * 4;
+    NB_REQUIRE(((uintptr_t)p.state | (uintptr_t)p.state_out) % 4 == 0, "linear attention: misaligned state");
+    if (p.state) check_extent(h, p.state, 0, state_bytes, "state");
+    if (p.state_out) check_extent(h, p.state_out, 0, state_bytes, "state_out");
+    p.B = d.batch; p.T = d.time_steps; p.H = d.heads; p.group = d.heads / d.key_heads;
+    p.dk = d.key_dim; p.dv = d.value_dim; p.scale = d.scale;
+    return p;
+}
+
+void LinAttnPlan::reserve() {}
+
+void LinAttnPlan::forward(const nb_linear_attention_io_t &io) {
+    const LinAttnParams p = params(io, false);
+    if (d.dtype == NB_DTYPE_BF16) launch_recurrent<__nv_bfloat16>(h, p);
+    else launch_recurrent<float>(h, p);
+}
+
+void LinAttnPlan::step(const nb_linear_attention_io_t &io) {
+    const LinAttnParams p = params(io, true);
+    if (d.dtype == NB_DTYPE_BF16) launch_step<__nv_bfloat16>(h, p);
+    else launch_step<float>(h, p);
+}
+
+}  // namespace nb

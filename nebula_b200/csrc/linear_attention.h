@@ -1,0 +1,75 @@
+// Linear attention with a decay for each head: the parameters its kernels share and the plan behind the C ABI.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "plans.h"
+
+namespace nb {
+
+// A tensor of tokens: element (b, t, head, i) at b * batch + t * token + head * head + i (packed: no batch term, t counted
+// from the sequence's first token in the tensor).
+struct TokenView {
+    const void *p;
+    long long batch, token, head;
+};
+
+struct LinAttnParams {
+    TokenView q, k, v, g, out;          // g: fp32 log decays, may be null; out is written
+    const int *offsets, *lengths, *slots;
+    long long tokens;                   // rows of packed tensors
+    const float *state;                 // [slot][head][key_dim][value_dim], may be null (zeros)
+    float *state_out;                   // may be null, may be `state`
+    long long state_slots;
+    int B, T, H, group;                 // group: value heads per query/key head
+    int dk, dv;
+    float scale;
+};
+
+// Where a sequence lies: its first row, its length, and its slot of the state (-1: not served, its rows of out are zeros).
+struct SeqAt {
+    long long first;
+    int len;
+    long long slot;
+};
+__device__ __forceinline__ SeqAt seq_at(const LinAttnParams &p, int b) {
+    SeqAt s;
+    s.first = 0;
+    s.len = p.T;
+    if (p.offsets) {
+        const long long lo = min(max((long long)p.offsets[b], 0LL), p.tokens), hi = min(max((long long)p.offsets[b + 1], lo), p.tokens);
+        s.first = lo;
+        s.len = (int)min(hi - lo, (long long)p.T);
+    } else if (p.lengths) {
+        s.len = min(max(p.lengths[b], 0), p.T);
+    }
+    s.slot = b;
+    if (p.slots) {
+        s.slot = p.slots[b];
+        if (s.slot < 0 || s.slot >= p.state_slots) s.slot = -1;
+    }
+    return s;
+}
+// Offset of a sequence's first token in a tensor, at a head.
+__device__ __forceinline__ long long token_base(const LinAttnParams &p, const TokenView &t, int b, const SeqAt &s, int head) {
+    return (p.offsets ? s.first * t.token : b * t.batch) + head * t.head;
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+struct LinAttnPlan : nb_plan_s {
+    nb_linear_attention_desc_t d;
+    DeviceBuffer ws;
+    LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc);
+    void forward(const nb_linear_attention_io_t &io);
+    void step(const nb_linear_attention_io_t &io);
+    void reserve();
+    size_t workspace_bytes() const override { return ws.n * sizeof(float); }
+    void output_dims(int dims[3]) const override { dims[0] = d.heads * d.value_dim; dims[1] = 1; dims[2] = 1; }
+    LinAttnParams params(const nb_linear_attention_io_t &io, bool step) const;
+};
+
+}  // namespace nb

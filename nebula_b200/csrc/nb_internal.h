@@ -299,6 +299,8 @@ struct SplitReduce {
     int pool;
 };
 void launch_splitk_reduce(nb_handle_s *h, const SplitReduce &p);
+// norms before and after a block with its gate and residual (norm_gate.cu); checks its arguments
+void launch_norm_gate(nb_handle_s *h, const nb_norm_gate_desc_t &d, const nb_norm_gate_io_t &io);
 // LSTM cell: z [B,4H] laid out [hidden unit][i,f,g,o] -> c_t, h_t (+ TF32-rounded copy of h_t)
 void launch_lstm_cell(nb_handle_s *h, const float *z, const float *c_prev, float *c_out, float *h_out,
                       float *h_round, int B, int H);

@@ -6,7 +6,7 @@
 
 #include "nb_internal.h"
 
-enum nb_plan_kind { NB_PLAN_CONV = 1, NB_PLAN_FC = 2, NB_PLAN_LSTM = 3, NB_PLAN_RNN = 4 };
+enum nb_plan_kind { NB_PLAN_CONV = 1, NB_PLAN_FC = 2, NB_PLAN_LSTM = 3, NB_PLAN_RNN = 4, NB_PLAN_LINEAR_ATTENTION = 5 };
 
 struct nb_plan_s {
     int kind;

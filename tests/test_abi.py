@@ -62,3 +62,16 @@ def test_product_never_touches_the_oracle():
     for path in list((ROOT / "nebula_b200").rglob("*.py")) + list((ROOT / "nebula_b200" / "csrc").glob("*")):
         if path.is_file():
             assert "oracle" not in path.read_text(errors="ignore"), f"{path} mentions the oracle"
+
+
+def test_packed_structs_have_the_header_s_layout(tmp_path):
+    """The binding fills three structs as plain bytes: their sizes and last members lie where the C compiler puts them."""
+    import subprocess
+    from nebula_b200 import api
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "nebula_b200.h"\nint main(void){printf("%zu %zu %zu %zu %zu\\n", sizeof(nb_linear_attention_io_t),'
+                   ' offsetof(nb_linear_attention_io_t, state_slots), sizeof(nb_norm_gate_desc_t), offsetof(nb_norm_gate_desc_t, x_stride),'
+                   ' sizeof(nb_norm_gate_io_t));return 0;}\n')
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "sizes")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [api._ATTENTION_IO.size, api._ATTENTION_IO.size - 8, api._NORM_DESC.size, 40, api._NORM_IO.size]
