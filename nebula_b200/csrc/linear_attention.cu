@@ -11,6 +11,7 @@ namespace nb {
 namespace {
 
 constexpr int MAX_DIM = 256;
+constexpr int RECURRENT_TOKENS = 16;        // prompts of up to so many tokens go token by token
 
 // ------------------------------------------------------------------ single tokens
 // S' = exp(g) S + k v^T and o = scale q^T S'.  Bound by the state, which is read and written once: 8 bytes a value for 5
@@ -206,6 +207,8 @@ LinAttnPlan::LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc)
     if (d.key_dim > MAX_DIM || d.value_dim > MAX_DIM) throw Error(NB_ERR_UNSUPPORTED, "linear attention: heads of more than 256 values");
     // grids are indexed in 31 bits, the smallest column tile being 16 wide
     NB_REQUIRE((long long)d.batch * d.heads * ((d.value_dim + 15) / 16) < (1LL << 31), "linear attention: too many sequences and heads");
+    chunked = linear_attention_chunks_supported(d) && d.time_steps > RECURRENT_TOKENS;
+    if (chunked) split = linear_attention_split(d, h->sm_count);
 }
 
 LinAttnParams LinAttnPlan::params(const nb_linear_attention_io_t &io, bool step) const {
@@ -257,10 +260,17 @@ LinAttnParams LinAttnPlan::params(const nb_linear_attention_io_t &io, bool step)
     return p;
 }
 
-void LinAttnPlan::reserve() {}
+void LinAttnPlan::reserve() {
+    if (chunked && split.n > 1) ws.reserve(linear_attention_workspace(d, split));
+}
 
 void LinAttnPlan::forward(const nb_linear_attention_io_t &io) {
     const LinAttnParams p = params(io, false);
+    if (chunked) {
+        reserve();
+        linear_attention_chunks(h, p, split, ws.p);
+        return;
+    }
     if (d.dtype == NB_DTYPE_BF16) launch_recurrent<__nv_bfloat16>(h, p);
     else launch_recurrent<float>(h, p);
 }

@@ -60,9 +60,18 @@ template <class T> __device__ __forceinline__ T from_f32(float x);
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Prompts in chunks on the tensor cores (linear_attention_chunk.cu): parts of the axis of tokens, and chunks of each.
+struct LinAttnSplit { int n, chunks; };
+bool linear_attention_chunks_supported(const nb_linear_attention_desc_t &d);
+LinAttnSplit linear_attention_split(const nb_linear_attention_desc_t &d, int sms);
+size_t linear_attention_workspace(const nb_linear_attention_desc_t &d, const LinAttnSplit &s);     // floats
+void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAttnSplit &split, float *ws);
+
 struct LinAttnPlan : nb_plan_s {
     nb_linear_attention_desc_t d;
-    DeviceBuffer ws;
+    DeviceBuffer ws;                    // states at the splits
+    bool chunked = false;
+    LinAttnSplit split = {1, 1};
     LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc);
     void forward(const nb_linear_attention_io_t &io);
     void step(const nb_linear_attention_io_t &io);

@@ -1,0 +1,745 @@
+// Linear attention over prompts in chunks of 64 tokens on the tensor cores (bf16 tensors, heads of up to 128 values).
+//
+// With positions i, j of a chunk, G_ij the sum of the log decays of tokens j+1 .. i, and S the state before the chunk:
+//   out_i = scale * [ sum_{j<=i} exp(G_ij) (q_i . k_j) v_j  +  exp(G_i) q_i^T S ],   G_i from the chunk's start
+//   S'    = exp(G_end) S + sum_j exp(G_end,j) k_j v_j^T
+// Everything is computed transposed, with the 128 accumulator lanes being the values of a head (or the keys j), because then both
+// products that weights have to be put into first take them from tensor memory, and the state keeps one lane's row in one thread:
+//   A^T [j][i]    = K Q^T                M = 128 (64 keys; the other rows read what lies behind and are dropped), N = 64
+//   O1^T [dv][i]  = V^T P^T              P = A masked and weighted, bf16, in shared memory
+//   O2^T [dv][i]  = S^T Q^T              S rounded to bf16, in tensor memory
+//   D^T [dv][dk]  = (V w)^T K            w_j = exp(G_end,j); V w in three bf16 terms, in tensor memory
+// The state itself is fp32, in the registers of eight warps, and so are all exponents.  What is rounded to bf16: P and the S that
+// the queries read (each a relative 2^-9 of a term of a sum whose result is rounded to bf16 anyway).  V w is not rounded: a
+// product of 24 bits is cut into three terms of 8, exactly, since the state is an fp32 result that lives on.
+// The weights are sums of log decays between two positions, so nothing overflows; decays of zero (log decay below -104, where exp
+// is 0 in fp32) are kept out of the sums and handled as a mask, so that the sums around them keep their precision.
+//
+// Bound by HBM where heads are 128 wide and there are as many sequences and heads as SMs: a chunk brings 64 KB and its MMAs are
+// worth 1400 cycles, against 2750 cycles that an SM's share of the bandwidth takes.
+//
+// A tensor core multiplies masked entries by zero, which is NaN for infinities and NaN in k and v.  Those are looked for on the
+// way, and a sequence that holds any is done again token by token (recurrence()).
+#include "linear_attention.h"
+#include "tc_common.cuh"
+
+namespace nb {
+
+using namespace tc;
+
+namespace {
+
+constexpr int C = 64;                       // tokens of a chunk
+constexpr int STATE_WARPS = 8, OUT_WARPS = 4, LOAD_WARPS = 2;
+constexpr int OUT0 = STATE_WARPS, LOAD0 = OUT0 + OUT_WARPS, MMA_WARP = LOAD0 + LOAD_WARPS;
+constexpr int THREADS = 32 * (MMA_WARP + 1);
+constexpr int HALF_TILE = C * 128;          // [64 tokens][64 values] of bf16, rows of 128 bytes, 128-byte swizzle
+constexpr int SLOTS = 8;                    // of the decays' ring: more than the stages of the tiles' plus two chunks
+constexpr int MAX_STAGES = 5;
+constexpr float RESET = -104.0f;            // exp of this and less is 0 in fp32
+// columns of tensor memory
+constexpr uint32_t T_KQ = 0, T_O2 = 64, T_O1 = 128, T_D = 192, T_S = 320, T_VW = 384, T_COLS = 512;
+
+// What the log decays of a chunk come to.
+struct Decays {
+    float sum2[C];              // from the chunk's start through the token, without resets, in powers of two
+    float from_start[C];        // exp of the same in powers of e, 0 behind a reset: the state's weight
+    float to_end[C];            // exp of the sum of the later tokens' log decays: the token's weight in the new state
+    unsigned resets[2];         // a bit per token
+    float less;                 // expm1 of the whole sum, -1 with a reset
+    float pad;
+};
+
+struct ChunkParams {
+    LinAttnParams a;
+    int splits, chunks_per_split;       // of the axis of tokens
+    float *ws;                          // [B*H][splits - 1][dk][dv]: states at the splits
+    float *ws_less;                     // [B*H][splits - 1]: expm1 of each split's log decay
+    int vec[3];                         // q, k, v: rows of whole 16-byte groups on 16-byte boundaries
+    int out_vec;
+    int stages;
+    int *status;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// bf16 operands, fp32 accumulators; a_mn, b_mn: the operand lies with its rows (M, N) contiguous instead of K
+__host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, int a_mn, int b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Shared-memory descriptor with 128-byte swizzle and groups of eight rows 1024 bytes apart.  K-major operands: eight M/N rows a
+// group.  M/N-major ones: eight K rows a group, and `mn_step` bytes to the next 64 M/N values.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t mn_step) {
+    return ((uint64_t)SMEM_DESC_HI << 32) | ((addr >> 4) & 0x3FFF) | ((mn_step >> 4) << 16);
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t *v) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// the upper halves of two words
+__device__ __forceinline__ uint32_t pack_high(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+
+// 16 bytes of a tile from a row that is not laid out in whole 16-byte groups
+__device__ __forceinline__ void copy_values(uint32_t dst, const __nv_bfloat16 *src, int n) {
+    const unsigned short *s = (const unsigned short *)src;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (2 * i < n ? s[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)s[2 * i + 1] << 16 : 0u);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+// Where a CTA works: a sequence and head, its tokens [first, first + n) and the state it starts from and ends in.
+struct Work {
+    SeqAt s;
+    int b, h, t0, n;
+    const float *from;          // nullptr: zeros
+    float *to;                  // nullptr: not wanted
+    bool states_only, skip;
+    int split;
+};
+template <bool STATES_ONLY>
+__device__ __forceinline__ Work work_of(const ChunkParams &p) {
+    Work w;
+    const int split = blockIdx.x % (STATES_ONLY ? p.splits - 1 : p.splits), bh = blockIdx.x / (STATES_ONLY ? p.splits - 1 : p.splits);
+    const long long size = (long long)p.a.dk * p.a.dv;
+    w.h = bh % p.a.H;
+    w.b = bh / p.a.H;
+    w.s = seq_at(p.a, w.b);
+    w.split = split;
+    const int span = p.chunks_per_split * C;
+    w.t0 = min(split * span, w.s.len);              // (split * span < T + span: no overflow, see the launch)
+    w.n = min(span, w.s.len - w.t0);
+    const bool last = w.t0 + w.n == w.s.len;
+    const long long at = (w.s.slot * p.a.H + w.h) * size;
+    float *mine = p.ws + ((long long)bh * (p.splits - 1) + split) * size;
+    if (STATES_ONLY) {
+        w.from = nullptr;
+        w.to = mine;
+        w.skip = last || w.s.slot < 0;              // nobody starts behind the last split
+    } else {
+        w.from = split ? mine - size : p.a.state ? p.a.state + at : nullptr;
+        w.to = last && p.a.state_out ? p.a.state_out + at : nullptr;
+        w.skip = split > 0 && w.n == 0;
+    }
+    return w;
+}
+
+// The recurrence as it is written, for a CTA's tokens: thread = column of the state, which lies in shared memory.
+template <bool STATES_ONLY>
+__device__ __noinline__ void recurrence(const ChunkParams &p, const Work &w, float *S) {
+    const int c = threadIdx.x;
+    if (c >= p.a.dv) return;
+    const LinAttnParams &a = p.a;
+    const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q.p + token_base(a, a.q, w.b, w.s, w.h / a.group);
+    const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group);
+    const __nv_bfloat16 *v = (const __nv_bfloat16 *)a.v.p + token_base(a, a.v, w.b, w.s, w.h) + c;
+    const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
+    __nv_bfloat16 *out = (__nv_bfloat16 *)a.out.p + token_base(a, a.out, w.b, w.s, w.h) + c;
+    for (int i = 0; i < a.dk; i++) S[i * 128 + c] = w.from ? w.from[(long long)i * a.dv + c] : 0.0f;
+    for (int t = w.t0; t < w.t0 + w.n; t++) {
+        const float less = g ? expm1f(g[t * a.g.token]) : 0.0f, x = to_f32(v[t * a.v.token]);
+        float o = 0.0f;
+        for (int i = 0; i < a.dk; i++) {
+            float s = S[i * 128 + c];
+            s = fmaf(to_f32(k[t * a.k.token + i]), x, less == -1.0f ? 0.0f : fmaf(less, s, s));
+            S[i * 128 + c] = s;
+            if (!STATES_ONLY) o = fmaf(to_f32(q[t * a.q.token + i]), s, o);
+        }
+        if (!STATES_ONLY) out[t * a.out.token] = from_f32<__nv_bfloat16>(a.scale * o);
+    }
+    if (w.to)
+        for (int i = 0; i < a.dk; i++) w.to[(long long)i * a.dv + c] = S[i * 128 + c];
+}
+
+// DK: 64 or 128, key_dim rounded up; tiles are padded with zeros.  STATES_ONLY: from zeros to the state behind each split but the
+// last, without queries and outputs.
+template <int DK, bool STATES_ONLY>
+__global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(const __grid_constant__ ChunkParams p) {
+    constexpr int KH = DK / 64;                         // half tiles of a key or query tile
+    constexpr int STAGE = (2 * KH + 2) * HALF_TILE;     // K, Q, V
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int stages = p.stages;
+    uint8_t *P = smem + stages * STAGE;                 // [2][64 keys][64 queries] bf16, swizzled like the tiles
+    __nv_bfloat16 *O = (__nv_bfloat16 *)(P + 2 * HALF_TILE);        // [64 queries][128]
+    Decays *dec = (Decays *)((uint8_t *)O + C * 128 * 2);
+    uint64_t *bars = (uint64_t *)(dec + SLOTS);
+    uint64_t *full = bars, *empty = bars + MAX_STAGES;  // loaders -> all, MMA -> loaders
+    uint64_t *kq_full = empty + MAX_STAGES, *kq_empty = kq_full + 1, *p_full = kq_empty + 1 /* [2] */, *o_full = p_full + 2, *o_empty = o_full + 1;
+    uint64_t *v_full = o_empty + 1, *d_full = v_full + 1, *s_full = d_full + 1, *s_empty = s_full + 1;
+    uint32_t *tmem_slot = (uint32_t *)(s_empty + 1);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    int *odd = (int *)(tmem_slot + 2);                  // infinities or NaN were met
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_dependents_start();
+    if (tid == 0) {
+        for (int s = 0; s < MAX_STAGES; s++) {
+            mbar_init(&full[s], 32 * LOAD_WARPS + 32);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(kq_full, 1);
+        mbar_init(kq_empty, 2);
+        mbar_init(&p_full[0], 2);
+        mbar_init(&p_full[1], 2);
+        mbar_init(o_full, 1);
+        mbar_init(o_empty, OUT_WARPS);
+        mbar_init(v_full, STATE_WARPS);
+        mbar_init(d_full, 1);
+        mbar_init(s_full, STATE_WARPS);
+        mbar_init(s_empty, 1);
+        *abort_flag = 0;
+        *odd = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(T_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // columns that no copy fills are zeros: of keys and queries past key_dim, of values past value_dim; and P's entries of keys behind
+    // all of a half's queries
+    if (p.a.dk < DK || p.a.dv % 64)
+        for (int i = tid; i < stages * STAGE / 16; i += THREADS) ((float4 *)smem)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!STATES_ONLY)
+        for (int i = tid; i < 2 * HALF_TILE / 16; i += THREADS) ((float4 *)P)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+
+    const LinAttnParams &a = p.a;
+    const Work w = work_of<STATES_ONLY>(p);
+    const bool served = w.s.slot >= 0 && !w.skip;
+    const int N = served ? (w.n + C - 1) / C : 0;
+    bool ok = true;
+
+    if (warp < STATE_WARPS) {
+        // ------------------------------------------------------------ the state, and V's weighted terms
+        const int quarter = warp & 3, half = warp >> 2, dv = quarter * 32 + lane;
+        const bool rows = quarter * 32 < a.dv, mine = dv < a.dv;
+        const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
+        constexpr int R = DK / 2;                       // columns of the state of a thread: keys half * R ...
+        float S[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int k = half * R + i;
+            S[i] = served && w.from && mine && k < a.dk ? w.from[(long long)k * a.dv + dv] : 0.0f;
+        }
+        auto put_state = [&]() {
+            uint32_t x[R / 2];
+#pragma unroll
+            for (int i = 0; i < R / 2; i++) x[i] = pack_bf16(S[2 * i], S[2 * i + 1]);
+            if constexpr (R == 64) tmem_st_32x32(at + T_S + half * 32, x);
+            else tmem_st_32x16(at + T_S + half * 16, x);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_full);
+        };
+        // this thread's column of V, weighted, for half of the chunk's tokens
+        float x[32], bad = 0.0f;
+        int stage = 0, slot = 0;
+        uint32_t phase = 0;
+        const uint32_t v_at = 2 * KH * HALF_TILE + (dv >> 6) * HALF_TILE + half * 32 * 128 + (dv & 7) * 2;
+        auto weigh = [&](int n) {
+            ok = ok && mbar_wait(&full[stage], phase, abort_flag, p.status);
+            if (ok && rows) {
+                const uint8_t *tile = smem + stage * STAGE + v_at;
+                const float *weight = dec[slot].to_end + half * 32;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 f = *(const float4 *)(weight + j);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const float v = __bfloat162float(*(const __nv_bfloat16 *)(tile + (j + u) * 128 + ((((dv >> 3) & 7) ^ ((j + u) & 7)) << 4)));
+                        const float by = u == 0 ? f.x : u == 1 ? f.y : u == 2 ? f.z : f.w;
+                        bad = fmaf(v, 0.0f, bad);
+                        x[j + u] = v * by;
+                    }
+                }
+            }
+            if (++stage == stages) stage = 0, phase ^= 1;
+            slot = (slot + 1) % SLOTS;
+        };
+        auto put_terms = [&]() {
+            uint32_t y[16];
+#pragma unroll
+            for (int term = 0; term < 3; term++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    y[j] = pack_high(x[2 * j], x[2 * j + 1]);
+                    x[2 * j] -= high_part(x[2 * j]);
+                    x[2 * j + 1] -= high_part(x[2 * j + 1]);
+                }
+                tmem_st_32x16(at + T_VW + term * 32 + half * 16, y);
+            }
+            tmem_st_wait();
+        };
+        if (N > 0) {
+            if (!STATES_ONLY) put_state();
+            weigh(0);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                put_terms();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_full);
+            }
+        }
+        for (int n = 0; n < N && ok; n++) {
+            const float less = dec[n % SLOTS].less;
+            if (n + 1 < N) weigh(n + 1);
+            ok = ok && mbar_wait(d_full, n & 1, abort_flag, p.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (n + 1 < N) put_terms();
+#pragma unroll
+            for (int c = 0; c < R; c += 32) {
+                uint32_t d[32];
+                tmem_ld_32x32(at + T_D + half * R + c, d);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    const float add = __uint_as_float(d[i]);
+                    // as S + (less S + add): what a decay near 1 takes away keeps its own precision
+                    S[c + i] = less == -1.0f ? add : S[c + i] + fmaf(less, S[c + i], add);
+                }
+            }
+            if (STATES_ONLY && mine)
+#pragma unroll
+                for (int i = 0; i < R; i++) bad = fmaf(S[i], 0.0f, bad);
+            if (n + 1 < N) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_full);
+                if (!STATES_ONLY) {
+                    ok = mbar_wait(s_empty, n & 1, abort_flag, p.status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    put_state();
+                }
+            }
+        }
+        if (bad != 0.0f) *odd = 1;
+        // (the last chunk's checks by the output warps come later: the state is stored behind the CTA's barrier)
+        tc_fence_before();
+        __syncthreads();
+        if (ok && served && w.to && mine && !*odd)
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int k = half * R + i;
+                if (k < a.dk) w.to[(long long)k * a.dv + dv] = S[i];
+            }
+    } else if (warp < LOAD0) {
+        // ------------------------------------------------------------ weights of pairs, outputs
+        const int quarter = warp - OUT0, t = tid - OUT0 * 32;
+        __nv_bfloat16 *out = (__nv_bfloat16 *)a.out.p + token_base(a, a.out, w.b, w.s, w.h);
+        if (!STATES_ONLY && w.s.slot < 0 && !w.skip)        // not served: zeros
+            for (int i = 0; i < w.n; i++)
+                for (int c = t; c < a.dv; c += 32 * OUT_WARPS) out[(w.t0 + i) * a.out.token + c] = from_f32<__nv_bfloat16>(0.0f);
+        if (!STATES_ONLY) {
+            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
+            int stage = 0;
+            uint32_t phase = 0;
+            auto pairs = [&](int n) {
+                ok = ok && mbar_wait(&full[stage], phase, abort_flag, p.status);
+                if (++stage == stages) stage = 0, phase ^= 1;
+                if (quarter >= 2) return;
+                ok = ok && mbar_wait(kq_full, n & 1, abort_flag, p.status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                tc_fence_after();
+                const Decays &d = dec[n % SLOTS];
+                const int j = quarter * 32 + lane;
+                const float mine = d.sum2[j];
+                // queries from j on up to the next reset behind j see key j
+                const unsigned long long later = ((unsigned long long)d.resets[1] << 32 | d.resets[0]) & (~0ULL << j << 1);
+                const int end = later ? __ffsll((long long)later) - 1 : C;
+                uint8_t *row = P + (n & 1) * HALF_TILE + j * 128;
+                for (int i0 = quarter * 32; i0 < C; i0 += 32) {
+                    uint32_t x[32];
+                    tmem_ld_32x32(at + T_KQ + i0, x);
+                    tmem_ld_wait();
+                    if (i0 == 32) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(kq_empty);
+                    }
+                    // infinities and NaN of a key make its whole row not finite
+                    if ((x[31] & 0x7f800000u) == 0x7f800000u) *odd = 1;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int i = i0 + c * 8 + e * 2;
+                            const float2 s = *(const float2 *)(d.sum2 + i);
+                            const float lo = i >= j && i < end ? __uint_as_float(x[c * 8 + e * 2]) * ex2(s.x - mine) : 0.0f;
+                            const float hi = i + 1 >= j && i + 1 < end ? __uint_as_float(x[c * 8 + e * 2 + 1]) * ex2(s.y - mine) : 0.0f;
+                            y[e] = pack_bf16(lo, hi);
+                        }
+                        *(uint4 *)(row + (((i0 / 8 + c) ^ (j & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[n & 1]);
+            };
+            if (N > 0) pairs(0);
+            ok = epilogue_all(ok, 1);
+            for (int n = 0; n < N && ok; n++) {
+                if (n + 1 < N) pairs(n + 1);
+                ok = ok && mbar_wait(o_full, n & 1, abort_flag, p.status);
+                ok = epilogue_all(ok, 1);               // (also: the slab of the chunk before has been read)
+                if (!ok) break;
+                tc_fence_after();
+                const float *weight = dec[n % SLOTS].from_start;
+                if (quarter * 32 < a.dv) {
+#pragma unroll 1
+                    for (int i0 = 0; i0 < C; i0 += 32) {
+                        uint32_t x[32], y[32];
+                        tmem_ld_32x32(at + T_O2 + i0, x);
+                        tmem_ld_32x32(at + T_O1 + i0, y);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const float e = weight[i0 + i], o1 = __uint_as_float(y[i]);
+                            const float o = e == 0.0f ? o1 : fmaf(e, __uint_as_float(x[i]), o1);
+                            O[(i0 + i) * 128 + t] = __float2bfloat16_rn(a.scale * o);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_empty);
+                epilogue_bar_sync(1);
+                const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
+                if (p.out_vec) {
+                    const int c = t & 15;
+                    if (c * 8 < a.dv)
+                        for (int i = t >> 4; i < m; i += 8) *(uint4 *)(out + (t0 + i) * a.out.token + c * 8) = *(const uint4 *)(O + i * 128 + c * 8);
+                } else if (t < a.dv) {
+                    for (int i = 0; i < m; i++) out[(t0 + i) * a.out.token + t] = O[i * 128 + t];
+                }
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+    } else if (warp < MMA_WARP) {
+        // ------------------------------------------------------------ loads
+        const int t = tid - LOAD0 * 32;
+        const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group);
+        const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q.p + token_base(a, a.q, w.b, w.s, w.h / a.group);
+        const __nv_bfloat16 *v = (const __nv_bfloat16 *)a.v.p + token_base(a, a.v, w.b, w.s, w.h);
+        const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
+        // rows of a tile: a thread copies one 16-byte group of every `step`-th row
+        auto tile = [&](uint32_t dst, const __nv_bfloat16 *src, long long token, int width, bool vec, int t0, int m) {
+            const int groups = (width + 7) / 8, per = groups > 8 ? 16 : 8, step = 32 * LOAD_WARPS / per;
+            const int c = t % per, n = min(8, width - c * 8);
+            if (c >= groups) return;
+            dst += (c >> 3) * HALF_TILE;
+            src += t0 * token + c * 8;
+#pragma unroll 8
+            for (int r = t / per; r < C; r += step) {
+                const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                if (vec) cp_async16(to, src + (r < m ? r * token : 0), r < m ? 2 * n : 0);
+                else copy_values(to, src + (r < m ? r * token : 0), r < m ? n : 0);
+            }
+        };
+        int stage = 0;
+        uint32_t phase = 0;
+        float total = 0.0f;
+        bool any = false;
+        float2 next = make_float2(0.0f, 0.0f);
+        auto decays = [&](int n) {              // of tokens 2 * lane and the one behind it, 0 past the end
+            const int i = n * C + 2 * lane;
+            float2 f = make_float2(0.0f, 0.0f);
+            if (g && i < w.n) f.x = g[(w.t0 + i) * a.g.token];
+            if (g && i + 1 < w.n) f.y = g[(w.t0 + i + 1) * a.g.token];
+            return f;
+        };
+        if (warp == LOAD0 && N > 0) next = decays(0);
+        for (int n = 0; n < N; n++) {
+            if (n >= stages) {
+                ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            const uint32_t base = smem_u32(smem + stage * STAGE);
+            const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
+            tile(base, k, a.k.token, a.dk, p.vec[1], t0, m);
+            if (!STATES_ONLY) tile(base + KH * HALF_TILE, q, a.q.token, a.dk, p.vec[0], t0, m);
+            tile(base + 2 * KH * HALF_TILE, v, a.v.token, a.dv, p.vec[2], t0, m);
+            if (p.vec[0] && p.vec[1] && p.vec[2]) {
+                cp_async_arrive(&full[stage]);
+            } else {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                mbar_arrive(&full[stage]);
+            }
+            if (warp == LOAD0) {
+                const float2 f = next;
+                if (n + 1 < N) next = decays(n + 1);
+                Decays &d = dec[n % SLOTS];
+                const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
+                const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
+                float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
+                    if (lane >= o) up += u;
+                    if (lane + o < 32) down += v2;
+                }
+                const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1);
+                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+                if (lane == 0) before = 0.0f;
+                if (lane == 31) behind = 0.0f;
+                const unsigned upto = 0xffffffffu >> (31 - lane), under = upto >> 1;        // lanes up to this one; below it
+                const bool reset_before = ((even | odds) & under) != 0, reset_behind = ((even | odds) & ~upto) != 0;
+                const float s0 = before + g0;
+                constexpr float LOG2E = 1.4426950408889634f;
+                *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0 * LOG2E, up * LOG2E);
+                *(float2 *)(d.from_start + 2 * lane) =
+                    make_float2(reset_before || r0 ? 0.0f : expf(s0), reset_before || r0 || r1 ? 0.0f : expf(up));
+                *(float2 *)(d.to_end + 2 * lane) = make_float2(reset_behind || r1 ? 0.0f : expf(behind + g1), reset_behind ? 0.0f : expf(behind));
+                // a bit per token from a bit per pair
+                unsigned long long bits = 0;
+                if ((even | odds) != 0 && lane == 0)
+                    for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
+                const float sum = __shfl_sync(0xffffffffu, up, 31);
+                if (lane == 0) {
+                    d.resets[0] = (unsigned)bits;
+                    d.resets[1] = (unsigned)(bits >> 32);
+                    d.less = (even | odds) ? -1.0f : expm1f(sum);
+                }
+                total += sum;
+                any = any || (even | odds) != 0;
+                mbar_arrive(&full[stage]);
+            }
+            if (++stage == stages) stage = 0, phase ^= 1;
+        }
+        if (STATES_ONLY && warp == LOAD0 && lane == 0 && served)
+            p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        tc_fence_before();
+        __syncthreads();
+    } else {
+        // ------------------------------------------------------------ MMAs, by one thread
+        if (lane == 0 && N > 0) {
+            int stage = 0, next_stage = 0;
+            uint32_t next_phase = 0;
+            const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0;
+            // the tiles of a chunk are there (written by copies and stores of other threads, read by MMAs)
+            auto arrived = [&]() {
+                ok = ok && mbar_wait(&full[next_stage], next_phase, abort_flag, p.status);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
+            };
+            auto keys_queries = [&](int s) {
+                const uint32_t k = smem_u32(smem + s * STAGE), q = k + KH * HALF_TILE;
+#pragma unroll
+                for (int i = 0; i < DK / 16; i++) {
+                    const uint32_t off = (i >> 2) * HALF_TILE + (i & 3) * 32;
+                    umma_bf16(tmem + T_KQ, tile_desc(k + off, 16), tile_desc(q + off, 16), idesc_bf16(128, C, 0, 0), i != 0);
+                }
+                umma_commit(kq_full);
+            };
+            arrived();
+            if (ok && !STATES_ONLY) keys_queries(0);
+            for (int n = 0; n < N && ok; n++) {
+                const uint32_t k = smem_u32(smem + stage * STAGE), q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
+                ok = mbar_wait(v_full, n & 1, abort_flag, p.status);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int term = 2; term >= 0; term--)
+#pragma unroll
+                    for (int i = 0; i < C / 16; i++)
+                        umma_bf16_ts(tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
+                                     idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
+                umma_commit(d_full);
+                if (n + 1 < N) {
+                    arrived();
+                    if (ok && !STATES_ONLY) {
+                        ok = mbar_wait(kq_empty, n & 1, abort_flag, p.status);
+                        tc_fence_after();
+                        if (ok) keys_queries(next_stage ? next_stage - 1 : stages - 1);
+                    }
+                }
+                if (!ok) break;
+                if (!STATES_ONLY) {
+                    ok = mbar_wait(s_full, n & 1, abort_flag, p.status) && (n == 0 || mbar_wait(o_empty, (n - 1) & 1, abort_flag, p.status));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < DK / 16; i++)
+                        umma_bf16_ts(tmem + T_O2, tmem + T_S + i * 8, tile_desc(q + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
+                                     idesc_bf16(128, C, 0, 0), i != 0);
+                    umma_commit(s_empty);
+                    ok = mbar_wait(&p_full[n & 1], n >> 1 & 1, abort_flag, p.status);
+                    if (!ok) break;
+                    const uint32_t pt = smem_u32(P + (n & 1) * HALF_TILE);
+#pragma unroll
+                    for (int i = 0; i < C / 16; i++)
+                        umma_bf16(tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE), idesc_bf16(128, C, 1, 1), i != 0);
+                    umma_commit(o_full);
+                }
+                umma_commit(&empty[stage]);
+                if (++stage == stages) stage = 0;
+            }
+        }
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+    }
+
+    // ---------------------------------------------------------------- teardown (every warp has passed the barrier above)
+    if (*abort_flag) {
+        // give copies and MMAs still in flight time to land before tensor memory is released
+        for (int i = 0; i < 64; i++) __nanosleep(2000);
+        __syncthreads();
+    }
+    if (warp == MMA_WARP) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(T_COLS) : "memory");
+    }
+    if (*odd && served && !*abort_flag) recurrence<STATES_ONLY>(p, w, (float *)smem);
+}
+
+// Turns the states that the splits came to by themselves into the states they start from.
+__global__ void __launch_bounds__(256) linear_attention_join_kernel(const __grid_constant__ ChunkParams p, int blocks) {
+    grid_begin();
+    const int bh = blockIdx.x / blocks, h = bh % p.a.H, b = bh / p.a.H;
+    const long long size = (long long)p.a.dk * p.a.dv;
+    const long long i = (long long)(blockIdx.x % blocks) * blockDim.x + threadIdx.x;
+    const SeqAt s = seq_at(p.a, b);
+    const int chunks = (s.len + C - 1) / C, n = (chunks + p.chunks_per_split - 1) / p.chunks_per_split - 1;     // splits but the last
+    if (i >= size || s.slot < 0) return;
+    float S = p.a.state ? p.a.state[(s.slot * p.a.H + h) * size + i] : 0.0f;
+    float *ws = p.ws + (long long)bh * (p.splits - 1) * size + i;
+    const float *less = p.ws_less + (long long)bh * (p.splits - 1);
+    for (int k = 0; k < n; k++) {
+        const float own = ws[k * size], l = less[k];
+        S = l == -1.0f ? own : S + fmaf(l, S, own);
+        ws[k * size] = S;
+    }
+}
+
+template <int DK>
+constexpr int stage_bytes() { return (2 * (DK / 64) + 2) * HALF_TILE; }
+template <int DK>
+constexpr int stages_of() { return DK == 128 ? 3 : MAX_STAGES; }
+template <int DK>
+constexpr size_t smem_bytes() { return 1024 + stages_of<DK>() * stage_bytes<DK>() + 2 * HALF_TILE + C * 128 * 2 + SLOTS * sizeof(Decays) + 256; }
+
+template <int DK, bool STATES_ONLY>
+void launch_chunks(nb_handle_s *h, const ChunkParams &p) {
+    static_assert(smem_bytes<DK>() <= 227 * 1024, "shared memory");
+    auto kernel = linear_attention_chunk_kernel<DK, STATES_ONLY>;
+    const unsigned bit = 1u << (DK / 64 - 1 + (STATES_ONLY ? 2 : 0));
+    if (!(h->linear_attention_ready & bit)) {
+        NB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<DK>()));
+        h->linear_attention_ready |= bit;
+    }
+    const int splits = STATES_ONLY ? p.splits - 1 : p.splits;
+    launch_overlapped(h, kernel, dim3((unsigned)(p.a.B * p.a.H * splits)), THREADS, smem_bytes<DK>(), p);
+    check_launch("linear_attention_chunk_kernel");
+    count_launch(h);
+}
+
+}  // namespace
+
+bool linear_attention_chunks_supported(const nb_linear_attention_desc_t &d) {
+    return d.dtype == NB_DTYPE_BF16 && d.key_dim <= 128 && d.value_dim <= 128;
+}
+
+// Parts that the axis of tokens is cut into where there are fewer sequences and heads than SMs.  Cutting costs a pass for the
+// states (which loads keys and values again; about 0.6 of a chunk's time) and two launches; a CTA's own start and end are worth
+// about 5 chunks.
+LinAttnSplit linear_attention_split(const nb_linear_attention_desc_t &d, int sms) {
+    const long long bh = (long long)d.batch * d.heads;
+    const int chunks = (d.time_steps + C - 1) / C;
+    LinAttnSplit best = {1, chunks};
+    double least = 1e30;
+    for (int s = 1; s <= 64 && s <= chunks && (s == 1 || bh * s <= 4LL * sms); s++) {
+        const int per = (chunks + s - 1) / s;
+        const int n = (chunks + per - 1) / per;         // what these parts come to
+        const double waves = (double)((bh * n + sms - 1) / sms), pre = (double)((bh * (n - 1) + sms - 1) / sms);
+        const double cost = waves * (per + 5.0) + (n > 1 ? pre * (0.6 * per + 5.0) + 4.0 : 0.0);
+        if (cost < least) {
+            least = cost;
+            best = {n, per};
+        }
+    }
+    return best;
+}
+size_t linear_attention_workspace(const nb_linear_attention_desc_t &d, const LinAttnSplit &s) {
+    return (size_t)d.batch * d.heads * (s.n - 1) * ((size_t)d.key_dim * d.value_dim + 1);
+}
+
+void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAttnSplit &split, float *ws) {
+    ChunkParams p = {};
+    p.a = a;
+    p.splits = split.n;
+    p.chunks_per_split = split.chunks;
+    p.ws = ws;
+    p.ws_less = ws + (size_t)a.B * a.H * (split.n - 1) * a.dk * a.dv;
+    p.status = h->d_status;
+    auto whole = [&](const TokenView &t, int dim, bool ragged) {
+        const long long strides = (a.offsets ? 0 : t.batch) | t.token | t.head;
+        return (uintptr_t)t.p % 16 == 0 && strides % 8 == 0 && (ragged || dim % 8 == 0);
+    };
+    // (a copy of the last values of a row may be shorter than 16 bytes; a store may not)
+    p.vec[0] = whole(a.q, a.dk, true);
+    p.vec[1] = whole(a.k, a.dk, true);
+    p.vec[2] = whole(a.v, a.dv, true);
+    p.out_vec = whole(a.out, a.dv, false);
+    const bool wide = a.dk > 64;
+    p.stages = wide ? stages_of<128>() : stages_of<64>();
+    if (p.splits > 1) {
+        if (wide) launch_chunks<128, true>(h, p);
+        else launch_chunks<64, true>(h, p);
+        const int blocks = (a.dk * a.dv + 255) / 256;
+        launch_overlapped(h, linear_attention_join_kernel, dim3((unsigned)(a.B * a.H * blocks)), 256, 0, p, blocks);
+        check_launch("linear_attention_join_kernel");
+        count_launch(h);
+    }
+    if (wide) launch_chunks<128, false>(h, p);
+    else launch_chunks<64, false>(h, p);
+}
+
+}  // namespace nb
