@@ -5,7 +5,7 @@
 //   S'    = exp(G_end) S + sum_j exp(G_end,j) k_j v_j^T
 // Everything is computed transposed, with the 128 accumulator lanes being the values of a head (or the keys j), because then both
 // products that weights have to be put into first take them from tensor memory, and the state keeps one lane's row in one thread:
-//   A^T [j][i]    = K Q^T                M = 128 (64 keys; the other rows read what lies behind and are dropped), N = 64
+//   A^T [j][i]    = K Q^T                M = 64, N = 64
 //   O1^T [dv][i]  = V^T P^T              P = A masked and weighted, bf16, in shared memory
 //   O2^T [dv][i]  = S^T Q^T              S rounded to bf16, in tensor memory
 //   D^T [dv][dk]  = (V w)^T K            w_j = exp(G_end,j); V w in three bf16 terms, in tensor memory
@@ -20,6 +20,9 @@
 //
 // A tensor core multiplies masked entries by zero, which is NaN for infinities and NaN in k and v.  Those are looked for on the
 // way, and a sequence that holds any is done again token by token (recurrence()).
+#include <cmath>
+#include <type_traits>
+
 #include "linear_attention.h"
 #include "tc_common.cuh"
 
@@ -31,7 +34,7 @@ namespace {
 
 constexpr int C = 64;                       // tokens of a chunk
 constexpr int STATE_WARPS = 8, OUT_WARPS = 4, LOAD_WARPS = 2;
-constexpr int OUT0 = STATE_WARPS, LOAD0 = OUT0 + OUT_WARPS, MMA_WARP = LOAD0 + LOAD_WARPS;
+constexpr int OUT0 = STATE_WARPS, LOAD0 = OUT0 + OUT_WARPS, DECAY_WARP = LOAD0 + LOAD_WARPS, MMA_WARP = DECAY_WARP + 1;
 constexpr int THREADS = 32 * (MMA_WARP + 1);
 constexpr int HALF_TILE = C * 128;          // [64 tokens][64 values] of bf16, rows of 128 bytes, 128-byte swizzle
 constexpr int SLOTS = 8;                    // of the decays' ring: more than the stages of the tiles' plus two chunks
@@ -43,7 +46,7 @@ constexpr uint32_t T_KQ = 0, T_O2 = 64, T_O1 = 128, T_D = 192, T_S = 320, T_VW =
 // What the log decays of a chunk come to.
 struct Decays {
     float sum2[C];              // from the chunk's start through the token, without resets, in powers of two
-    float from_start[C];        // exp of the same in powers of e, 0 behind a reset: the state's weight
+    float from_start[C];        // scale times exp of the same in powers of e, 0 behind a reset: the state's weight
     float to_end[C];            // exp of the sum of the later tokens' log decays: the token's weight in the new state
     unsigned resets[2];         // a bit per token
     float less;                 // expm1 of the whole sum, -1 with a reset
@@ -57,6 +60,8 @@ struct ChunkParams {
     float *ws_less;                     // [B*H][splits - 1]: expm1 of each split's log decay
     int vec[3];                         // q, k, v: rows of whole 16-byte groups on 16-byte boundaries
     int out_vec;
+    float scale, log2_size;             // and the logarithm of its size
+    unsigned negative;                  // scale < 0
     int stages;
     int *status;
 };
@@ -100,6 +105,70 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t *v)
         "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
         : "memory");
 }
+// 16 lanes of tensor memory in the layout of matrix fragments: thread t holds rows t / 4 and t / 4 + 8.  Loads: of every eight columns
+// 2 (t % 4) and the next one, of both rows; stores of four columns: column t % 4, of both rows.
+__device__ __forceinline__ void tmem_ld_16x256_x8(uint32_t taddr, uint32_t (&v)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t *v) {
+    __syncwarp();
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr)
+                 : "memory");
+}
+// four 8 x 8 matrices of 16-bit values: lane t gives the address of row t % 8 of matrix t / 8
+__device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t *v) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void stmatrix(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void stmatrix_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// two fp32 operations at once
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 as_float2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+// a half word of ones for each of the two lowest bits
+__device__ __forceinline__ uint32_t two_halves(unsigned bits) { return (bits & 1) * 0xffffu | (bits >> 1 & 1) * 0xffff0000u; }
+// mbar_wait with its loop out of line: a kernel of many waits does not fit the instruction caches otherwise
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
+    return mbar_wait(bar, parity, abort_flag, status);
+}
+__device__ __forceinline__ bool mbar_wait_far(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
+    return mbar_try_wait(bar, parity) || mbar_wait_long(smem_u32(bar), parity, abort_flag, status);
+}
+__device__ __forceinline__ float low_value(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_value(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -191,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stages = p.stages;
     uint8_t *P = smem + stages * STAGE;                 // [2][64 keys][64 queries] bf16, swizzled like the tiles
-    __nv_bfloat16 *O = (__nv_bfloat16 *)(P + 2 * HALF_TILE);        // [64 queries][128]
+    __nv_bfloat16 *O = (__nv_bfloat16 *)(P + 2 * HALF_TILE);        // [64 queries][128], groups of eight values at (group ^ query % 8)
     Decays *dec = (Decays *)((uint8_t *)O + C * 128 * 2);
     uint64_t *bars = (uint64_t *)(dec + SLOTS);
     uint64_t *full = bars, *empty = bars + MAX_STAGES;  // loaders -> all, MMA -> loaders
@@ -209,9 +278,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             mbar_init(&empty[s], 1);
         }
         mbar_init(kq_full, 1);
-        mbar_init(kq_empty, 2);
-        mbar_init(&p_full[0], 2);
-        mbar_init(&p_full[1], 2);
+        mbar_init(kq_empty, OUT_WARPS);
+        mbar_init(&p_full[0], OUT_WARPS);
+        mbar_init(&p_full[1], OUT_WARPS);
         mbar_init(o_full, 1);
         mbar_init(o_empty, OUT_WARPS);
         mbar_init(v_full, STATE_WARPS);
@@ -251,118 +320,111 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         const bool rows = quarter * 32 < a.dv, mine = dv < a.dv;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
         constexpr int R = DK / 2;                       // columns of the state of a thread: keys half * R ...
-        float S[R];
+        float2 S[R / 2];
 #pragma unroll
         for (int i = 0; i < R; i++) {
             const int k = half * R + i;
-            S[i] = served && w.from && mine && k < a.dk ? w.from[(long long)k * a.dv + dv] : 0.0f;
+            (&S[i / 2].x)[i & 1] = served && w.from && mine && k < a.dk ? w.from[(long long)k * a.dv + dv] : 0.0f;
         }
-        auto put_state = [&]() {
-            uint32_t x[R / 2];
-#pragma unroll
-            for (int i = 0; i < R / 2; i++) x[i] = pack_bf16(S[2 * i], S[2 * i + 1]);
-            if constexpr (R == 64) tmem_st_32x32(at + T_S + half * 32, x);
-            else tmem_st_32x16(at + T_S + half * 16, x);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_full);
-        };
-        // this thread's column of V, weighted, for half of the chunk's tokens
-        float x[32], bad = 0.0f;
-        int stage = 0, slot = 0;
+        // V [dv][token] of half of the chunk's tokens, in pairs of tokens and in the layout of fragments: [16 dv][8 tokens][dv, dv + 8]
+        uint32_t v[16];
+        float2 by[4];
+        int stage = 0;
         uint32_t phase = 0;
-        const uint32_t v_at = 2 * KH * HALF_TILE + (dv >> 6) * HALF_TILE + half * 32 * 128 + (dv & 7) * 2;
-        auto weigh = [&](int n) {
-            ok = ok && mbar_wait(&full[stage], phase, abort_flag, p.status);
-            if (ok && rows) {
-                const uint8_t *tile = smem + stage * STAGE + v_at;
-                const float *weight = dec[slot].to_end + half * 32;
+        const uint32_t v_at = smem_u32(smem) + 2 * KH * HALF_TILE + (quarter >> 1) * HALF_TILE + (half * 32 + (lane >> 4) * 8 + (lane & 7)) * 128;
+        // chunk n's state while chunk n + 1's values are prepared
+#pragma unroll 1
+        for (int n = -1; n < N; n++) {
+            const bool more = n + 1 < N;
+            if (more) {
+                ok = mbar_wait_far(&full[stage], phase, abort_flag, p.status);
+                if (ok && rows) {
+                    const uint32_t tile = v_at + stage * STAGE;
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 f = *(const float4 *)(weight + j);
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const float v = __bfloat162float(*(const __nv_bfloat16 *)(tile + (j + u) * 128 + ((((dv >> 3) & 7) ^ ((j + u) & 7)) << 4)));
-                        const float by = u == 0 ? f.x : u == 1 ? f.y : u == 2 ? f.z : f.w;
-                        bad = fmaf(v, 0.0f, bad);
-                        x[j + u] = v * by;
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t group = ((((quarter & 1) * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
+                        ldmatrix_trans(tile + group, v + h * 8);
+                        ldmatrix_trans(tile + group + 16 * 128, v + h * 8 + 4);
                     }
-                }
-            }
-            if (++stage == stages) stage = 0, phase ^= 1;
-            slot = (slot + 1) % SLOTS;
-        };
-        auto put_terms = [&]() {
-            uint32_t y[16];
 #pragma unroll
-            for (int term = 0; term < 3; term++) {
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    y[j] = pack_high(x[2 * j], x[2 * j + 1]);
-                    x[2 * j] -= high_part(x[2 * j]);
-                    x[2 * j + 1] -= high_part(x[2 * j + 1]);
+                    for (int t = 0; t < 4; t++) by[t] = *(const float2 *)(dec[(n + 1) % SLOTS].to_end + half * 32 + t * 8 + (lane & 3) * 2);
                 }
-                tmem_st_32x16(at + T_VW + term * 32 + half * 16, y);
+                if (++stage == stages) stage = 0, phase ^= 1;
             }
-            tmem_st_wait();
-        };
-        if (N > 0) {
-            if (!STATES_ONLY) put_state();
-            weigh(0);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-                put_terms();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(v_full);
-            }
-        }
-        for (int n = 0; n < N && ok; n++) {
-            const float less = dec[n % SLOTS].less;
-            if (n + 1 < N) weigh(n + 1);
-            ok = ok && mbar_wait(d_full, n & 1, abort_flag, p.status);
+            if (n >= 0) ok = ok && mbar_wait_far(d_full, n & 1, abort_flag, p.status);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            if (n + 1 < N) put_terms();
+            if (more && rows) {
 #pragma unroll
-            for (int c = 0; c < R; c += 32) {
-                uint32_t d[32];
-                tmem_ld_32x32(at + T_D + half * R + c, d);
-                tmem_ld_wait();
+                for (int h = 0; h < 2; h++) {
+                    float2 x[8];
+                    uint32_t y[8];
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    const float add = __uint_as_float(d[i]);
-                    // as S + (less S + add): what a decay near 1 takes away keeps its own precision
-                    S[c + i] = less == -1.0f ? add : S[c + i] + fmaf(less, S[c + i], add);
+                    for (int i = 0; i < 8; i++) x[i] = mul2(make_float2(low_value(v[h * 8 + i]), high_value(v[h * 8 + i])), by[i / 2]);
+#pragma unroll
+                    for (int term = 0; term < 3; term++) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            y[i] = pack_high(x[i].x, x[i].y);
+                            if (term < 2) x[i] = fma2(make_float2(-1.0f, -1.0f), make_float2(high_part(x[i].x), high_part(x[i].y)), x[i]);
+                        }
+                        tmem_st_16x128_x4(at + ((uint32_t)(h * 16) << 16) + T_VW + term * 32 + half * 16, y);
+                    }
                 }
             }
-            if (STATES_ONLY && mine)
+            if (n >= 0) {
+                const float less = dec[n % SLOTS].less;
 #pragma unroll
-                for (int i = 0; i < R; i++) bad = fmaf(S[i], 0.0f, bad);
-            if (n + 1 < N) {
+                for (int c = 0; c < R; c += 32) {
+                    uint32_t d[32];
+                    tmem_ld_32x32(at + T_D + half * R + c, d);
+                    tmem_ld_wait();
+                    // as S + (less S + new): what a decay near 1 takes away keeps its own precision.  Once a value is not finite it
+                    // stays so, whatever the decays
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        float2 &x = S[c / 2 + i];
+                        x = add2(x, fma2(make_float2(less, less), x, make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]))));
+                    }
+                }
+            }
+            if (more) {
+                tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_full);
                 if (!STATES_ONLY) {
-                    ok = mbar_wait(s_empty, n & 1, abort_flag, p.status);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    put_state();
+                    uint32_t x[R / 2];
+#pragma unroll
+                    for (int i = 0; i < R / 2; i++) x[i] = pack_bf16(S[i].x, S[i].y);
+                    if (n >= 0) {
+                        ok = mbar_wait_far(s_empty, n & 1, abort_flag, p.status);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    if constexpr (R == 64) tmem_st_32x32(at + T_S + half * 32, x);
+                    else tmem_st_32x16(at + T_S + half * 16, x);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_full);
                 }
             }
         }
-        if (bad != 0.0f) *odd = 1;
-        // (the last chunk's checks by the output warps come later: the state is stored behind the CTA's barrier)
+        // infinities and NaN, of the first state, keys or values, are in the last state whatever the decays were
+        float bad = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R / 2; i++) bad = fmaf(S[i].x, 0.0f, fmaf(S[i].y, 0.0f, bad));
+        if (mine && bad != 0.0f) *odd = 1;
         tc_fence_before();
         __syncthreads();
         if (ok && served && w.to && mine && !*odd)
 #pragma unroll
             for (int i = 0; i < R; i++) {
                 const int k = half * R + i;
-                if (k < a.dk) w.to[(long long)k * a.dv + dv] = S[i];
+                if (k < a.dk) w.to[(long long)k * a.dv + dv] = (&S[i / 2].x)[i & 1];
             }
     } else if (warp < LOAD0) {
         // ------------------------------------------------------------ weights of pairs, outputs
@@ -375,71 +437,74 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
             int stage = 0;
             uint32_t phase = 0;
-            auto pairs = [&](int n) {
-                ok = ok && mbar_wait(&full[stage], phase, abort_flag, p.status);
-                if (++stage == stages) stage = 0, phase ^= 1;
-                if (quarter >= 2) return;
-                ok = ok && mbar_wait(kq_full, n & 1, abort_flag, p.status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                tc_fence_after();
-                const Decays &d = dec[n % SLOTS];
-                const int j = quarter * 32 + lane;
-                const float mine = d.sum2[j];
-                // queries from j on up to the next reset behind j see key j
-                const unsigned long long later = ((unsigned long long)d.resets[1] << 32 | d.resets[0]) & (~0ULL << j << 1);
-                const int end = later ? __ffsll((long long)later) - 1 : C;
-                uint8_t *row = P + (n & 1) * HALF_TILE + j * 128;
-                for (int i0 = quarter * 32; i0 < C; i0 += 32) {
-                    uint32_t x[32];
-                    tmem_ld_32x32(at + T_KQ + i0, x);
-                    tmem_ld_wait();
-                    if (i0 == 32) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(kq_empty);
-                    }
-                    // infinities and NaN of a key make its whole row not finite
-                    if ((x[31] & 0x7f800000u) == 0x7f800000u) *odd = 1;
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t y[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int i = i0 + c * 8 + e * 2;
-                            const float2 s = *(const float2 *)(d.sum2 + i);
-                            const float lo = i >= j && i < end ? __uint_as_float(x[c * 8 + e * 2]) * ex2(s.x - mine) : 0.0f;
-                            const float hi = i + 1 >= j && i + 1 < end ? __uint_as_float(x[c * 8 + e * 2 + 1]) * ex2(s.y - mine) : 0.0f;
-                            y[e] = pack_bf16(lo, hi);
-                        }
-                        *(uint4 *)(row + (((i0 / 8 + c) ^ (j & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
+            // chunk n's weights of pairs, then chunk n - 1's outputs
+#pragma unroll 1
+            for (int n = 0; n <= N; n++) {
+                if (n < N) {
+                    ok = ok && mbar_wait_far(&full[stage], phase, abort_flag, p.status) && mbar_wait_far(kq_full, n & 1, abort_flag, p.status);
+                    if (++stage == stages) stage = 0, phase ^= 1;
+                    ok = __all_sync(0xffffffffu, ok);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[n & 1]);
-            };
-            if (N > 0) pairs(0);
-            ok = epilogue_all(ok, 1);
-            for (int n = 0; n < N && ok; n++) {
-                if (n + 1 < N) pairs(n + 1);
-                ok = ok && mbar_wait(o_full, n & 1, abort_flag, p.status);
-                ok = epilogue_all(ok, 1);               // (also: the slab of the chunk before has been read)
+                if (n < N && ok) {
+                    tc_fence_after();
+                    // keys j and j + 8, against queries 8 g + 2 (lane % 4) and the next one; the 16 queries from 16 * quarter on are
+                    // on the diagonal, those before see none of the keys
+                    uint32_t x[32];
+                    tmem_ld_16x256_x8(at + T_KQ, x);
+                    const Decays &d = dec[n % SLOTS];
+                    const int j = quarter * 16 + (lane >> 2), i1 = 2 * (lane & 3);
+                    const float m0 = p.log2_size - d.sum2[j], m1 = p.log2_size - d.sum2[j + 8];
+                    const unsigned long long resets = (unsigned long long)d.resets[1] << 32 | d.resets[0];
+                    // queries that see each key: from its own token on up to the next reset behind it
+                    const unsigned long long from0 = ~0ULL << j, from1 = ~0ULL << (j + 8), r0 = resets & from0 << 1, r1 = resets & from1 << 1;
+                    const unsigned long long see0 = (r0 & -r0) - 1 & from0, see1 = (r1 & -r1) - 1 & from1;
+                    const uint32_t row = smem_u32(P) + (n & 1) * HALF_TILE + (quarter * 16 + (lane & 15)) * 128;
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(kq_empty);
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        if (g >= 2 * quarter) {
+                            const float2 s = *(const float2 *)(d.sum2 + g * 8 + i1);
+                            x[4 * g] = pack_bf16(__uint_as_float(x[4 * g]) * ex2(s.x + m0), __uint_as_float(x[4 * g + 1]) * ex2(s.y + m0));
+                            x[4 * g + 1] = pack_bf16(__uint_as_float(x[4 * g + 2]) * ex2(s.x + m1), __uint_as_float(x[4 * g + 3]) * ex2(s.y + m1));
+                            if (g < 2 * quarter + 2 || resets != 0) {
+                                x[4 * g] &= two_halves((unsigned)(see0 >> (g * 8 + i1)));
+                                x[4 * g + 1] &= two_halves((unsigned)(see1 >> (g * 8 + i1)));
+                            }
+                            if (g & 1) stmatrix(row + (((g - 1 + (lane >> 4)) ^ (lane & 7)) << 4), x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[n & 1]);
+                }
+                if (n == 0) continue;
+                const int before = n - 1;
+                ok = ok && mbar_wait_far(o_full, before & 1, abort_flag, p.status);
+                ok = epilogue_all(ok, 1);               // (also: the outputs of the chunk before that have left shared memory)
                 if (!ok) break;
                 tc_fence_after();
-                const float *weight = dec[n % SLOTS].from_start;
                 if (quarter * 32 < a.dv) {
-#pragma unroll 1
-                    for (int i0 = 0; i0 < C; i0 += 32) {
+                    const float *weight = dec[before % SLOTS].from_start + 2 * (lane & 3);
+                    const uint32_t to = smem_u32(O) + ((lane >> 4) * 8 + (lane & 7)) * 256;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {       // 16 values of the head
                         uint32_t x[32], y[32];
-                        tmem_ld_32x32(at + T_O2 + i0, x);
-                        tmem_ld_32x32(at + T_O1 + i0, y);
+                        tmem_ld_16x256_x8(at + ((uint32_t)(h * 16) << 16) + T_O2, x);
+                        tmem_ld_16x256_x8(at + ((uint32_t)(h * 16) << 16) + T_O1, y);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const float e = weight[i0 + i], o1 = __uint_as_float(y[i]);
-                            const float o = e == 0.0f ? o1 : fmaf(e, __uint_as_float(x[i]), o1);
-                            O[(i0 + i) * 128 + t] = __float2bfloat16_rn(a.scale * o);
+                        for (int g = 0; g < 8; g++) {
+                            const float2 e = *(const float2 *)(weight + g * 8);
+                            const float2 o0 = fma2(e, as_float2(x[4 * g], x[4 * g + 1]), as_float2(y[4 * g], y[4 * g + 1]));
+                            const float2 o1 = fma2(e, as_float2(x[4 * g + 2], x[4 * g + 3]), as_float2(y[4 * g + 2], y[4 * g + 3]));
+                            x[4 * g] = pack_bf16(o0.x, o0.y);
+                            x[4 * g + 1] = pack_bf16(o1.x, o1.y);
+                            if (g & 1)
+                                stmatrix_trans(to + (g - 1) * 8 * 256 + (((quarter * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4), x[4 * g - 4],
+                                               x[4 * g - 3], x[4 * g], x[4 * g + 1]);
                         }
                     }
                 }
@@ -447,39 +512,83 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_empty);
                 epilogue_bar_sync(1);
-                const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
+                const int t0 = w.t0 + before * C, m = min(C, w.n - before * C);
                 if (p.out_vec) {
                     const int c = t & 15;
-                    if (c * 8 < a.dv)
-                        for (int i = t >> 4; i < m; i += 8) *(uint4 *)(out + (t0 + i) * a.out.token + c * 8) = *(const uint4 *)(O + i * 128 + c * 8);
+                    if (c * 8 < a.dv) {
+                        const __nv_bfloat16 *from = O + (t >> 4) * 128 + ((c ^ (t >> 4)) << 3);
+                        __nv_bfloat16 *to = out + (t0 + (t >> 4)) * a.out.token + c * 8;
+                        if (m == C) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++, to += 8 * a.out.token) *(uint4 *)to = *(const uint4 *)(from + i * 8 * 128);
+                        } else {
+                            for (int i = t >> 4; i < m; i += 8, to += 8 * a.out.token, from += 8 * 128) *(uint4 *)to = *(const uint4 *)from;
+                        }
+                    }
                 } else if (t < a.dv) {
-                    for (int i = 0; i < m; i++) out[(t0 + i) * a.out.token + t] = O[i * 128 + t];
+                    for (int i = 0; i < m; i++) out[(t0 + i) * a.out.token + t] = O[i * 128 + (((t >> 3) ^ (i & 7)) << 3) + (t & 7)];
                 }
             }
         }
         tc_fence_before();
         __syncthreads();
-    } else if (warp < MMA_WARP) {
+    } else if (warp < DECAY_WARP) {
         // ------------------------------------------------------------ loads
         const int t = tid - LOAD0 * 32;
         const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group);
         const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q.p + token_base(a, a.q, w.b, w.s, w.h / a.group);
         const __nv_bfloat16 *v = (const __nv_bfloat16 *)a.v.p + token_base(a, a.v, w.b, w.s, w.h);
-        const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
         // rows of a tile: a thread copies one 16-byte group of every `step`-th row
-        auto tile = [&](uint32_t dst, const __nv_bfloat16 *src, long long token, int width, bool vec, int t0, int m) {
-            const int groups = (width + 7) / 8, per = groups > 8 ? 16 : 8, step = 32 * LOAD_WARPS / per;
-            const int c = t % per, n = min(8, width - c * 8);
-            if (c >= groups) return;
-            dst += (c >> 3) * HALF_TILE;
-            src += t0 * token + c * 8;
-#pragma unroll 8
-            for (int r = t / per; r < C; r += step) {
-                const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                if (vec) cp_async16(to, src + (r < m ? r * token : 0), r < m ? 2 * n : 0);
-                else copy_values(to, src + (r < m ? r * token : 0), r < m ? n : 0);
+        auto tile = [&](auto groups_of, uint32_t dst, const __nv_bfloat16 *src, long long token, int width, bool vec, int t0, int m) {
+            constexpr int PER = decltype(groups_of)::value, STEP = 32 * LOAD_WARPS / PER;       // 4 or 8
+            const int c = t % PER, r0 = t / PER, n = min(8, width - c * 8);
+            if (n <= 0) return;
+            // the swizzle of row r0 + i * STEP: that of r0, with its upper bit inverted for the odd ones of steps of four
+            const uint32_t at[2] = {dst + (c >> 3) * HALF_TILE + r0 * 128 + (((c & 7) ^ r0) << 4),
+                                    dst + (c >> 3) * HALF_TILE + r0 * 128 + (((c & 7) ^ (r0 + STEP & 7)) << 4)};
+            src += (t0 + r0) * token + c * 8;
+            if (vec && m == C) {
+#pragma unroll
+                for (int i = 0; i < C / STEP; i++, src += STEP * token) cp_async16(at[i & 1] + i * STEP * 128, src, 2 * n);
+            } else {
+                const __nv_bfloat16 *any = src - r0 * token;            // rows past the end: nothing is read, zeros arrive
+#pragma unroll 4
+                for (int i = 0; i < C / STEP; i++, src += STEP * token) {
+                    const bool in = r0 + i * STEP < m;
+                    if (vec) cp_async16(at[i & 1] + i * STEP * 128, in ? src : any, in ? 2 * n : 0);
+                    else copy_values(at[i & 1] + i * STEP * 128, in ? src : any, in ? n : 0);
+                }
             }
         };
+        using Keys = std::integral_constant<int, DK / 8>;
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int n = 0; n < N; n++) {
+            if (n >= stages) {
+                ok = mbar_wait_far(&empty[stage], phase ^ 1, abort_flag, p.status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            const uint32_t base = smem_u32(smem + stage * STAGE);
+            const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
+            tile(Keys(), base, k, a.k.token, a.dk, p.vec[1], t0, m);
+            if (!STATES_ONLY) tile(Keys(), base + KH * HALF_TILE, q, a.q.token, a.dk, p.vec[0], t0, m);
+            if (a.dv > 64) tile(std::integral_constant<int, 16>(), base + 2 * KH * HALF_TILE, v, a.v.token, a.dv, p.vec[2], t0, m);
+            else tile(std::integral_constant<int, 8>(), base + 2 * KH * HALF_TILE, v, a.v.token, a.dv, p.vec[2], t0, m);
+            if (p.vec[0] && p.vec[1] && p.vec[2]) {
+                cp_async_arrive(&full[stage]);
+            } else {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                mbar_arrive(&full[stage]);
+            }
+            if (++stage == stages) stage = 0, phase ^= 1;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        tc_fence_before();
+        __syncthreads();
+    } else if (warp == DECAY_WARP) {
+        // ------------------------------------------------------------ decays
+        const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
         int stage = 0;
         uint32_t phase = 0;
         float total = 0.0f;
@@ -492,68 +601,54 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             if (g && i + 1 < w.n) f.y = g[(w.t0 + i + 1) * a.g.token];
             return f;
         };
-        if (warp == LOAD0 && N > 0) next = decays(0);
+        if (N > 0) next = decays(0);
         for (int n = 0; n < N; n++) {
             if (n >= stages) {
-                ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status);
+                ok = mbar_wait_far(&empty[stage], phase ^ 1, abort_flag, p.status);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
             }
-            const uint32_t base = smem_u32(smem + stage * STAGE);
-            const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
-            tile(base, k, a.k.token, a.dk, p.vec[1], t0, m);
-            if (!STATES_ONLY) tile(base + KH * HALF_TILE, q, a.q.token, a.dk, p.vec[0], t0, m);
-            tile(base + 2 * KH * HALF_TILE, v, a.v.token, a.dv, p.vec[2], t0, m);
-            if (p.vec[0] && p.vec[1] && p.vec[2]) {
-                cp_async_arrive(&full[stage]);
-            } else {
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                mbar_arrive(&full[stage]);
-            }
-            if (warp == LOAD0) {
-                const float2 f = next;
-                if (n + 1 < N) next = decays(n + 1);
-                Decays &d = dec[n % SLOTS];
-                const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
-                const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
-                float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
+            const float2 f = next;
+            if (n + 1 < N) next = decays(n + 1);
+            Decays &d = dec[n % SLOTS];
+            const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
+            const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
+            float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
-                    if (lane >= o) up += u;
-                    if (lane + o < 32) down += v2;
-                }
-                const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1);
-                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-                if (lane == 0) before = 0.0f;
-                if (lane == 31) behind = 0.0f;
-                const unsigned upto = 0xffffffffu >> (31 - lane), under = upto >> 1;        // lanes up to this one; below it
-                const bool reset_before = ((even | odds) & under) != 0, reset_behind = ((even | odds) & ~upto) != 0;
-                const float s0 = before + g0;
-                constexpr float LOG2E = 1.4426950408889634f;
-                *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0 * LOG2E, up * LOG2E);
-                *(float2 *)(d.from_start + 2 * lane) =
-                    make_float2(reset_before || r0 ? 0.0f : expf(s0), reset_before || r0 || r1 ? 0.0f : expf(up));
-                *(float2 *)(d.to_end + 2 * lane) = make_float2(reset_behind || r1 ? 0.0f : expf(behind + g1), reset_behind ? 0.0f : expf(behind));
-                // a bit per token from a bit per pair
-                unsigned long long bits = 0;
-                if ((even | odds) != 0 && lane == 0)
-                    for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
-                const float sum = __shfl_sync(0xffffffffu, up, 31);
-                if (lane == 0) {
-                    d.resets[0] = (unsigned)bits;
-                    d.resets[1] = (unsigned)(bits >> 32);
-                    d.less = (even | odds) ? -1.0f : expm1f(sum);
-                }
-                total += sum;
-                any = any || (even | odds) != 0;
-                mbar_arrive(&full[stage]);
+            for (int o = 1; o < 32; o <<= 1) {
+                const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
+                if (lane >= o) up += u;
+                if (lane + o < 32) down += v2;
             }
+            const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1);
+            float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+            if (lane == 0) before = 0.0f;
+            if (lane == 31) behind = 0.0f;
+            const unsigned upto = 0xffffffffu >> (31 - lane), under = upto >> 1;        // lanes up to this one; below it
+            const bool reset_before = ((even | odds) & under) != 0, reset_behind = ((even | odds) & ~upto) != 0;
+            const float s0 = before + g0;
+            constexpr float LOG2E = 1.4426950408889634f;
+            *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0 * LOG2E, up * LOG2E);
+            *(float2 *)(d.from_start + 2 * lane) =
+                make_float2(reset_before || r0 ? 0.0f : p.scale * expf(s0), reset_before || r0 || r1 ? 0.0f : p.scale * expf(up));
+            *(float2 *)(d.to_end + 2 * lane) = make_float2(reset_behind || r1 ? 0.0f : expf(behind + g1), reset_behind ? 0.0f : expf(behind));
+            // a bit per token from a bit per pair
+            unsigned long long bits = 0;
+            if ((even | odds) != 0 && lane == 0)
+                for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
+            const float sum = __shfl_sync(0xffffffffu, up, 31);
+            if (lane == 0) {
+                d.resets[0] = (unsigned)bits;
+                d.resets[1] = (unsigned)(bits >> 32);
+                d.less = (even | odds) ? -1.0f : expm1f(sum);
+            }
+            total += sum;
+            any = any || (even | odds) != 0;
+            mbar_arrive(&full[stage]);
             if (++stage == stages) stage = 0, phase ^= 1;
         }
-        if (STATES_ONLY && warp == LOAD0 && lane == 0 && served)
+        if (STATES_ONLY && lane == 0 && served)
             p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
-        asm volatile("cp.async.wait_all;" ::: "memory");
         tc_fence_before();
         __syncthreads();
     } else {
@@ -562,46 +657,43 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             int stage = 0, next_stage = 0;
             uint32_t next_phase = 0;
             const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0;
-            // the tiles of a chunk are there (written by copies and stores of other threads, read by MMAs)
-            auto arrived = [&]() {
-                ok = ok && mbar_wait(&full[next_stage], next_phase, abort_flag, p.status);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
-            };
-            auto keys_queries = [&](int s) {
-                const uint32_t k = smem_u32(smem + s * STAGE), q = k + KH * HALF_TILE;
-#pragma unroll
-                for (int i = 0; i < DK / 16; i++) {
-                    const uint32_t off = (i >> 2) * HALF_TILE + (i & 3) * 32;
-                    umma_bf16(tmem + T_KQ, tile_desc(k + off, 16), tile_desc(q + off, 16), idesc_bf16(128, C, 0, 0), i != 0);
-                }
-                umma_commit(kq_full);
-            };
-            arrived();
-            if (ok && !STATES_ONLY) keys_queries(0);
-            for (int n = 0; n < N && ok; n++) {
+            const uint32_t negative = p.negative << 13;         // of A: a negative scale
+#pragma unroll 1
+            for (int n = -1; n < N && ok; n++) {
                 const uint32_t k = smem_u32(smem + stage * STAGE), q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
-                ok = mbar_wait(v_full, n & 1, abort_flag, p.status);
-                if (!ok) break;
-                tc_fence_after();
+                if (n >= 0) {
+                    ok = mbar_wait_far(v_full, n & 1, abort_flag, p.status);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
-                for (int term = 2; term >= 0; term--)
+                    for (int term = 2; term >= 0; term--)
 #pragma unroll
-                    for (int i = 0; i < C / 16; i++)
-                        umma_bf16_ts(tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
-                                     idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
-                umma_commit(d_full);
-                if (n + 1 < N) {
-                    arrived();
-                    if (ok && !STATES_ONLY) {
-                        ok = mbar_wait(kq_empty, n & 1, abort_flag, p.status);
-                        tc_fence_after();
-                        if (ok) keys_queries(next_stage ? next_stage - 1 : stages - 1);
-                    }
+                        for (int i = 0; i < C / 16; i++)
+                            umma_bf16_ts(tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
+                                         idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
+                    umma_commit(d_full);
                 }
-                if (!ok) break;
+                if (n + 1 < N) {
+                    // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
+                    ok = mbar_wait_far(&full[next_stage], next_phase, abort_flag, p.status);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (!STATES_ONLY) {
+                        ok = ok && (n < 0 || mbar_wait_far(kq_empty, n & 1, abort_flag, p.status));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t k1 = smem_u32(smem + next_stage * STAGE), q1 = k1 + KH * HALF_TILE;
+#pragma unroll
+                        for (int i = 0; i < DK / 16; i++) {
+                            const uint32_t off = (i >> 2) * HALF_TILE + (i & 3) * 32;
+                            umma_bf16(tmem + T_KQ, tile_desc(k1 + off, 16), tile_desc(q1 + off, 16), idesc_bf16(64, C, 0, 0), i != 0);
+                        }
+                        umma_commit(kq_full);
+                    }
+                    if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
+                }
+                if (n < 0) continue;
                 if (!STATES_ONLY) {
-                    ok = mbar_wait(s_full, n & 1, abort_flag, p.status) && (n == 0 || mbar_wait(o_empty, (n - 1) & 1, abort_flag, p.status));
+                    ok = mbar_wait_far(s_full, n & 1, abort_flag, p.status) && (n == 0 || mbar_wait_far(o_empty, (n - 1) & 1, abort_flag, p.status));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
@@ -609,12 +701,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                         umma_bf16_ts(tmem + T_O2, tmem + T_S + i * 8, tile_desc(q + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
                                      idesc_bf16(128, C, 0, 0), i != 0);
                     umma_commit(s_empty);
-                    ok = mbar_wait(&p_full[n & 1], n >> 1 & 1, abort_flag, p.status);
+                    ok = mbar_wait_far(&p_full[n & 1], n >> 1 & 1, abort_flag, p.status);
                     if (!ok) break;
                     const uint32_t pt = smem_u32(P + (n & 1) * HALF_TILE);
 #pragma unroll
                     for (int i = 0; i < C / 16; i++)
-                        umma_bf16(tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE), idesc_bf16(128, C, 1, 1), i != 0);
+                        umma_bf16(tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE),
+                                  idesc_bf16(128, C, 1, 1) | negative, i != 0);
                     umma_commit(o_full);
                 }
                 umma_commit(&empty[stage]);
@@ -719,6 +812,9 @@ void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAt
     p.ws = ws;
     p.ws_less = ws + (size_t)a.B * a.H * (split.n - 1) * a.dk * a.dv;
     p.status = h->d_status;
+    p.scale = a.scale;
+    p.log2_size = std::log2(std::fabs(a.scale));
+    p.negative = a.scale < 0.0f;
     auto whole = [&](const TokenView &t, int dim, bool ragged) {
         const long long strides = (a.offsets ? 0 : t.batch) | t.token | t.head;
         return (uintptr_t)t.p % 16 == 0 && strides % 8 == 0 && (ragged || dim % 8 == 0);
