@@ -158,15 +158,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 __device__ __forceinline__ float2 as_float2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
-// a half word of ones for each of the two lowest bits
-__device__ __forceinline__ uint32_t two_halves(unsigned bits) { return (bits & 1) * 0xffffu | (bits >> 1 & 1) * 0xffff0000u; }
-// mbar_wait with its loop out of line: a kernel of many waits does not fit the instruction caches otherwise
-__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    return mbar_wait(bar, parity, abort_flag, status);
+// Bounded waits, with the loop out of line: the roles' loops have to fit the instruction caches together.  A wait that runs out sets
+// the abort flag, and every wait of the CTA then returns at once: the roles run through what is left, on whatever they find.
+__device__ __noinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
+    mbar_wait(bar, parity, abort_flag, status);
 }
-__device__ __forceinline__ bool mbar_wait_far(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    return mbar_try_wait(bar, parity) || mbar_wait_long(smem_u32(bar), parity, abort_flag, status);
-}
+struct Waits {
+    volatile int *abort_flag;
+    int *status;
+    __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const {
+        if (!mbar_try_wait(bar, parity)) wait_long(smem_u32(bar), parity, abort_flag, status);
+        __syncwarp();
+    }
+};
 __device__ __forceinline__ float low_value(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_value(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -312,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     const Work w = work_of<STATES_ONLY>(p);
     const bool served = w.s.slot >= 0 && !w.skip;
     const int N = served ? (w.n + C - 1) / C : 0;
-    bool ok = true;
+    const Waits wait = {abort_flag, p.status};
 
     if (warp < STATE_WARPS) {
         // ------------------------------------------------------------ the state, and V's weighted terms
@@ -337,8 +341,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         for (int n = -1; n < N; n++) {
             const bool more = n + 1 < N;
             if (more) {
-                ok = mbar_wait_far(&full[stage], phase, abort_flag, p.status);
-                if (ok && rows) {
+                wait(&full[stage], phase);
+                if (rows) {
                     const uint32_t tile = v_at + stage * STAGE;
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -351,9 +355,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 }
                 if (++stage == stages) stage = 0, phase ^= 1;
             }
-            if (n >= 0) ok = ok && mbar_wait_far(d_full, n & 1, abort_flag, p.status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            if (n >= 0) wait(d_full, n & 1);
             tc_fence_after();
             if (more && rows) {
 #pragma unroll
@@ -398,12 +400,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     uint32_t x[R / 2];
 #pragma unroll
                     for (int i = 0; i < R / 2; i++) x[i] = pack_bf16(S[i].x, S[i].y);
-                    if (n >= 0) {
-                        ok = mbar_wait_far(s_empty, n & 1, abort_flag, p.status);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
+                    if (n >= 0) wait(s_empty, n & 1);
+                    tc_fence_after();
                     if constexpr (R == 64) tmem_st_32x32(at + T_S + half * 32, x);
                     else tmem_st_32x16(at + T_S + half * 16, x);
                     tmem_st_wait();
@@ -420,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         if (mine && bad != 0.0f) *odd = 1;
         tc_fence_before();
         __syncthreads();
-        if (ok && served && w.to && mine && !*odd)
+        if (served && w.to && mine && !*odd && !*abort_flag)
 #pragma unroll
             for (int i = 0; i < R; i++) {
                 const int k = half * R + i;
@@ -432,32 +430,29 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         __nv_bfloat16 *out = (__nv_bfloat16 *)a.out.p + token_base(a, a.out, w.b, w.s, w.h);
         if (!STATES_ONLY && w.s.slot < 0 && !w.skip)        // not served: zeros
             for (int i = 0; i < w.n; i++)
+#pragma unroll 1
                 for (int c = t; c < a.dv; c += 32 * OUT_WARPS) out[(w.t0 + i) * a.out.token + c] = from_f32<__nv_bfloat16>(0.0f);
         if (!STATES_ONLY) {
             const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
             int stage = 0;
             uint32_t phase = 0;
+            // of a pair's 16 x 16 tokens on the diagonal: queries 2 (lane % 4) and the next one against key lane / 4, of the same eight
+            const int r = lane >> 2, i1 = 2 * (lane & 3);
+            const uint32_t causal = (i1 >= r ? 0xffffu : 0u) | (i1 + 1 >= r ? 0xffff0000u : 0u);
             // chunk n's weights of pairs, then chunk n - 1's outputs
 #pragma unroll 1
             for (int n = 0; n <= N; n++) {
                 if (n < N) {
-                    ok = ok && mbar_wait_far(&full[stage], phase, abort_flag, p.status) && mbar_wait_far(kq_full, n & 1, abort_flag, p.status);
+                    wait(&full[stage], phase);
                     if (++stage == stages) stage = 0, phase ^= 1;
-                    ok = __all_sync(0xffffffffu, ok);
-                }
-                if (n < N && ok) {
+                    wait(kq_full, n & 1);
                     tc_fence_after();
-                    // keys j and j + 8, against queries 8 g + 2 (lane % 4) and the next one; the 16 queries from 16 * quarter on are
-                    // on the diagonal, those before see none of the keys
+                    // keys r and r + 8 of the 16 of this warp, against the queries from its first key on: 8 g + i1 and the next one
+                    // (columns past the last query are not used)
                     uint32_t x[32];
-                    tmem_ld_16x256_x8(at + T_KQ, x);
+                    tmem_ld_16x256_x8(at + T_KQ + quarter * 16, x);
                     const Decays &d = dec[n % SLOTS];
-                    const int j = quarter * 16 + (lane >> 2), i1 = 2 * (lane & 3);
-                    const float m0 = p.log2_size - d.sum2[j], m1 = p.log2_size - d.sum2[j + 8];
-                    const unsigned long long resets = (unsigned long long)d.resets[1] << 32 | d.resets[0];
-                    // queries that see each key: from its own token on up to the next reset behind it
-                    const unsigned long long from0 = ~0ULL << j, from1 = ~0ULL << (j + 8), r0 = resets & from0 << 1, r1 = resets & from1 << 1;
-                    const unsigned long long see0 = (r0 & -r0) - 1 & from0, see1 = (r1 & -r1) - 1 & from1;
+                    const float m0 = p.log2_size - d.sum2[quarter * 16 + r], m1 = p.log2_size - d.sum2[quarter * 16 + r + 8];
                     const uint32_t row = smem_u32(P) + (n & 1) * HALF_TILE + (quarter * 16 + (lane & 15)) * 128;
                     tmem_ld_wait();
                     tc_fence_before();
@@ -465,16 +460,22 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     if (lane == 0) mbar_arrive(kq_empty);
 #pragma unroll
                     for (int g = 0; g < 8; g++) {
-                        if (g >= 2 * quarter) {
-                            const float2 s = *(const float2 *)(d.sum2 + g * 8 + i1);
-                            x[4 * g] = pack_bf16(__uint_as_float(x[4 * g]) * ex2(s.x + m0), __uint_as_float(x[4 * g + 1]) * ex2(s.y + m0));
-                            x[4 * g + 1] = pack_bf16(__uint_as_float(x[4 * g + 2]) * ex2(s.x + m1), __uint_as_float(x[4 * g + 3]) * ex2(s.y + m1));
-                            if (g < 2 * quarter + 2 || resets != 0) {
-                                x[4 * g] &= two_halves((unsigned)(see0 >> (g * 8 + i1)));
-                                x[4 * g + 1] &= two_halves((unsigned)(see1 >> (g * 8 + i1)));
-                            }
-                            if (g & 1) stmatrix(row + (((g - 1 + (lane >> 4)) ^ (lane & 7)) << 4), x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
-                        }
+                        if (g % 2 == 0 && g >= 8 - 2 * quarter) break;
+                        const float2 s = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + i1);
+                        x[4 * g] = pack_bf16(__uint_as_float(x[4 * g]) * ex2(s.x + m0), __uint_as_float(x[4 * g + 1]) * ex2(s.y + m0));
+                        x[4 * g + 1] = pack_bf16(__uint_as_float(x[4 * g + 2]) * ex2(s.x + m1), __uint_as_float(x[4 * g + 3]) * ex2(s.y + m1));
+                        if (g == 0) x[0] &= causal, x[1] = 0;
+                        if (g == 1) x[5] &= causal;
+                        if (g & 1)
+                            stmatrix(row + (((quarter * 2 + g - 1 + (lane >> 4)) ^ (lane & 7)) << 4), x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
+                    }
+                    if (d.resets[0] | d.resets[1]) {        // a key is not seen from the next reset behind it on
+                        __syncwarp();
+                        const int j = quarter * 16 + (lane & 15);
+                        const unsigned long long later = ((unsigned long long)d.resets[1] << 32 | d.resets[0]) & (~0ULL << j << 1);
+#pragma unroll 1
+                        for (int i = later ? __ffsll((long long)later) - 1 + (lane >> 4) : C; i < C; i += 2)
+                            *(__nv_bfloat16 *)(P + (n & 1) * HALF_TILE + j * 128 + (((i >> 3) ^ (j & 7)) << 4) + (i & 7) * 2) = from_f32<__nv_bfloat16>(0.0f);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -482,15 +483,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 }
                 if (n == 0) continue;
                 const int before = n - 1;
-                ok = ok && mbar_wait_far(o_full, before & 1, abort_flag, p.status);
-                ok = epilogue_all(ok, 1);               // (also: the outputs of the chunk before that have left shared memory)
-                if (!ok) break;
+                wait(o_full, before & 1);
+                epilogue_bar_sync(1);                       // the outputs of the chunk before have left shared memory
                 tc_fence_after();
                 if (quarter * 32 < a.dv) {
-                    const float *weight = dec[before % SLOTS].from_start + 2 * (lane & 3);
-                    const uint32_t to = smem_u32(O) + ((lane >> 4) * 8 + (lane & 7)) * 256;
-#pragma unroll
+                    const float *weight = dec[before % SLOTS].from_start + i1;
+#pragma unroll 1
                     for (int h = 0; h < 2; h++) {       // 16 values of the head
+                        const uint32_t to = smem_u32(O) + ((lane >> 4) * 8 + (lane & 7)) * 256 + (((quarter * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
                         uint32_t x[32], y[32];
                         tmem_ld_16x256_x8(at + ((uint32_t)(h * 16) << 16) + T_O2, x);
                         tmem_ld_16x256_x8(at + ((uint32_t)(h * 16) << 16) + T_O1, y);
@@ -502,9 +502,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                             const float2 o1 = fma2(e, as_float2(x[4 * g + 2], x[4 * g + 3]), as_float2(y[4 * g + 2], y[4 * g + 3]));
                             x[4 * g] = pack_bf16(o0.x, o0.y);
                             x[4 * g + 1] = pack_bf16(o1.x, o1.y);
-                            if (g & 1)
-                                stmatrix_trans(to + (g - 1) * 8 * 256 + (((quarter * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4), x[4 * g - 4],
-                                               x[4 * g - 3], x[4 * g], x[4 * g + 1]);
+                            if (g & 1) stmatrix_trans(to + (g - 1) * 8 * 256, x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
                         }
                     }
                 }
@@ -522,10 +520,12 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
 #pragma unroll
                             for (int i = 0; i < 8; i++, to += 8 * a.out.token) *(uint4 *)to = *(const uint4 *)(from + i * 8 * 128);
                         } else {
+#pragma unroll 1
                             for (int i = t >> 4; i < m; i += 8, to += 8 * a.out.token, from += 8 * 128) *(uint4 *)to = *(const uint4 *)from;
                         }
                     }
                 } else if (t < a.dv) {
+#pragma unroll 1
                     for (int i = 0; i < m; i++) out[(t0 + i) * a.out.token + t] = O[i * 128 + (((t >> 3) ^ (i & 7)) << 3) + (t & 7)];
                 }
             }
@@ -534,48 +534,54 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         __syncthreads();
     } else if (warp < DECAY_WARP) {
         // ------------------------------------------------------------ loads
+        // A thread copies one 16-byte group of every `step`-th row of a tile, 64 / step times.
         const int t = tid - LOAD0 * 32;
-        const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group);
-        const __nv_bfloat16 *q = (const __nv_bfloat16 *)a.q.p + token_base(a, a.q, w.b, w.s, w.h / a.group);
-        const __nv_bfloat16 *v = (const __nv_bfloat16 *)a.v.p + token_base(a, a.v, w.b, w.s, w.h);
-        // rows of a tile: a thread copies one 16-byte group of every `step`-th row
-        auto tile = [&](auto groups_of, uint32_t dst, const __nv_bfloat16 *src, long long token, int width, bool vec, int t0, int m) {
-            constexpr int PER = decltype(groups_of)::value, STEP = 32 * LOAD_WARPS / PER;       // 4 or 8
-            const int c = t % PER, r0 = t / PER, n = min(8, width - c * 8);
-            if (n <= 0) return;
-            // the swizzle of row r0 + i * STEP: that of r0, with its upper bit inverted for the odd ones of steps of four
-            const uint32_t at[2] = {dst + (c >> 3) * HALF_TILE + r0 * 128 + (((c & 7) ^ r0) << 4),
-                                    dst + (c >> 3) * HALF_TILE + r0 * 128 + (((c & 7) ^ (r0 + STEP & 7)) << 4)};
-            src += (t0 + r0) * token + c * 8;
-            if (vec && m == C) {
-#pragma unroll
-                for (int i = 0; i < C / STEP; i++, src += STEP * token) cp_async16(at[i & 1] + i * STEP * 128, src, 2 * n);
-            } else {
-                const __nv_bfloat16 *any = src - r0 * token;            // rows past the end: nothing is read, zeros arrive
-#pragma unroll 4
-                for (int i = 0; i < C / STEP; i++, src += STEP * token) {
-                    const bool in = r0 + i * STEP < m;
-                    if (vec) cp_async16(at[i & 1] + i * STEP * 128, in ? src : any, in ? 2 * n : 0);
-                    else copy_values(at[i & 1] + i * STEP * 128, in ? src : any, in ? n : 0);
-                }
-            }
-        };
-        using Keys = std::integral_constant<int, DK / 8>;
+        const bool all_vec = p.vec[0] && p.vec[1] && p.vec[2];
         int stage = 0;
         uint32_t phase = 0;
+#pragma unroll 1
         for (int n = 0; n < N; n++) {
-            if (n >= stages) {
-                ok = mbar_wait_far(&empty[stage], phase ^ 1, abort_flag, p.status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+            if (n >= stages) wait(&empty[stage], phase ^ 1);
+            const int m = min(C, w.n - n * C);
+#pragma unroll 1
+            for (int which = STATES_ONLY ? 1 : 0; which < 3; which++) {     // q, k, v
+                const TokenView &view = which == 0 ? a.q : which == 1 ? a.k : a.v;
+                const int width = which == 2 ? a.dv : a.dk, per = width > 64 ? 16 : 8, step = 32 * LOAD_WARPS / per;
+                const int c = t & (per - 1), r0 = t / per, bytes = 2 * min(8, width - c * 8);
+                if (bytes <= 0) continue;
+                // the swizzle of row r0 + i * step: that of r0, with its upper bit inverted for the odd ones of steps of four
+                const uint32_t dst = smem_u32(smem + stage * STAGE + (which == 2 ? 2 * KH : which == 0 ? KH : 0) * HALF_TILE + (c >> 3) * HALF_TILE) + r0 * 128;
+                uint32_t d0 = dst + (((c & 7) ^ r0) << 4), d1 = dst + step * 128 + (((c & 7) ^ (r0 + step & 7)) << 4);
+                const long long token = view.token * 2;
+                const char *first = (const char *)view.p + 2 * token_base(a, view, w.b, w.s, which == 2 ? w.h : w.h / a.group) +
+                                    (w.t0 + n * C) * token + c * 16;
+                const char *src = first + r0 * token;
+                if (p.vec[which] && m == C) {
+#pragma unroll 1
+                    for (int i = 0; i < per; i += 8) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            cp_async16(d0, src, bytes);
+                            src += step * token;
+                            cp_async16(d1, src, bytes);
+                            src += step * token;
+                            d0 += step * 256;
+                            d1 += step * 256;
+                        }
+                    }
+                } else {                    // of rows past the end nothing is read, zeros arrive
+#pragma unroll 1
+                    for (int r = r0; r < C; r += step) {
+                        if (p.vec[which]) cp_async16(d0, r < m ? src : first, r < m ? bytes : 0);
+                        else copy_values(d0, (const __nv_bfloat16 *)(r < m ? src : first), r < m ? bytes / 2 : 0);
+                        src += step * token;
+                        const uint32_t next = d0 + step * 256;
+                        d0 = d1;
+                        d1 = next;
+                    }
+                }
             }
-            const uint32_t base = smem_u32(smem + stage * STAGE);
-            const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
-            tile(Keys(), base, k, a.k.token, a.dk, p.vec[1], t0, m);
-            if (!STATES_ONLY) tile(Keys(), base + KH * HALF_TILE, q, a.q.token, a.dk, p.vec[0], t0, m);
-            if (a.dv > 64) tile(std::integral_constant<int, 16>(), base + 2 * KH * HALF_TILE, v, a.v.token, a.dv, p.vec[2], t0, m);
-            else tile(std::integral_constant<int, 8>(), base + 2 * KH * HALF_TILE, v, a.v.token, a.dv, p.vec[2], t0, m);
-            if (p.vec[0] && p.vec[1] && p.vec[2]) {
+            if (all_vec) {
                 cp_async_arrive(&full[stage]);
             } else {
                 asm volatile("cp.async.wait_all;" ::: "memory");
@@ -603,11 +609,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         };
         if (N > 0) next = decays(0);
         for (int n = 0; n < N; n++) {
-            if (n >= stages) {
-                ok = mbar_wait_far(&empty[stage], phase ^ 1, abort_flag, p.status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-            }
+            if (n >= stages) wait(&empty[stage], phase ^ 1);
             const float2 f = next;
             if (n + 1 < N) next = decays(n + 1);
             Decays &d = dec[n % SLOTS];
@@ -635,6 +637,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             // a bit per token from a bit per pair
             unsigned long long bits = 0;
             if ((even | odds) != 0 && lane == 0)
+#pragma unroll 1
                 for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
             const float sum = __shfl_sync(0xffffffffu, up, 31);
             if (lane == 0) {
@@ -658,14 +661,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             uint32_t next_phase = 0;
             const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0;
             const uint32_t negative = p.negative << 13;         // of A: a negative scale
+            auto wait1 = [&](uint64_t *bar, uint32_t parity) {
+                if (!mbar_try_wait(bar, parity)) wait_long(smem_u32(bar), parity, abort_flag, p.status);
+            };
 #pragma unroll 1
-            for (int n = -1; n < N && ok; n++) {
+            for (int n = -1; n < N; n++) {
                 const uint32_t k = smem_u32(smem + stage * STAGE), q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
                 if (n >= 0) {
-                    ok = mbar_wait_far(v_full, n & 1, abort_flag, p.status);
-                    if (!ok) break;
+                    wait1(v_full, n & 1);
                     tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                     for (int term = 2; term >= 0; term--)
 #pragma unroll
                         for (int i = 0; i < C / 16; i++)
@@ -675,34 +680,35 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 }
                 if (n + 1 < N) {
                     // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
-                    ok = mbar_wait_far(&full[next_stage], next_phase, abort_flag, p.status);
+                    wait1(&full[next_stage], next_phase);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     if (!STATES_ONLY) {
-                        ok = ok && (n < 0 || mbar_wait_far(kq_empty, n & 1, abort_flag, p.status));
-                        if (!ok) break;
+                        if (n >= 0) wait1(kq_empty, n & 1);
                         tc_fence_after();
-                        const uint32_t k1 = smem_u32(smem + next_stage * STAGE), q1 = k1 + KH * HALF_TILE;
+                        const uint32_t k1 = smem_u32(smem + next_stage * STAGE);
+#pragma unroll 1
+                        for (int h = 0; h < KH; h++)
 #pragma unroll
-                        for (int i = 0; i < DK / 16; i++) {
-                            const uint32_t off = (i >> 2) * HALF_TILE + (i & 3) * 32;
-                            umma_bf16(tmem + T_KQ, tile_desc(k1 + off, 16), tile_desc(q1 + off, 16), idesc_bf16(64, C, 0, 0), i != 0);
-                        }
+                            for (int i = 0; i < 4; i++)
+                                umma_bf16(tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
+                                          idesc_bf16(64, C, 0, 0), (h | i) != 0);
                         umma_commit(kq_full);
                     }
                     if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
                 }
                 if (n < 0) continue;
                 if (!STATES_ONLY) {
-                    ok = mbar_wait_far(s_full, n & 1, abort_flag, p.status) && (n == 0 || mbar_wait_far(o_empty, (n - 1) & 1, abort_flag, p.status));
-                    if (!ok) break;
+                    wait1(s_full, n & 1);
+                    if (n > 0) wait1(o_empty, (n - 1) & 1);
                     tc_fence_after();
+#pragma unroll 1
+                    for (int h = 0; h < KH; h++)
 #pragma unroll
-                    for (int i = 0; i < DK / 16; i++)
-                        umma_bf16_ts(tmem + T_O2, tmem + T_S + i * 8, tile_desc(q + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
-                                     idesc_bf16(128, C, 0, 0), i != 0);
+                        for (int i = 0; i < 4; i++)
+                            umma_bf16_ts(tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
+                                         idesc_bf16(128, C, 0, 0), (h | i) != 0);
                     umma_commit(s_empty);
-                    ok = mbar_wait_far(&p_full[n & 1], n >> 1 & 1, abort_flag, p.status);
-                    if (!ok) break;
+                    wait1(&p_full[n & 1], n >> 1 & 1);
                     const uint32_t pt = smem_u32(P + (n & 1) * HALF_TILE);
 #pragma unroll
                     for (int i = 0; i < C / 16; i++)
