@@ -36,6 +36,9 @@ constexpr int C = 64;                       // tokens of a chunk
 constexpr int STATE_WARPS = 8, OUT_WARPS = 4, LOAD_WARPS = 2;
 constexpr int OUT0 = STATE_WARPS, LOAD0 = OUT0 + OUT_WARPS, DECAY_WARP = LOAD0 + LOAD_WARPS, MMA_WARP = DECAY_WARP + 1;
 constexpr int THREADS = 32 * (MMA_WARP + 1);
+// Registers of a thread: what a launch of so many threads gets, and how the warpgroups share it (their sum is at most four times that)
+constexpr int REGS = 128, STATE_REGS = 160, OUT_REGS = 128, OTHER_REGS = 64;
+static_assert(THREADS == 512 && 2 * STATE_REGS + OUT_REGS + OTHER_REGS <= 4 * REGS, "registers");
 constexpr int HALF_TILE = C * 128;          // [64 tokens][64 values] of bf16, rows of 128 bytes, 128-byte swizzle
 constexpr int SLOTS = 8;                    // of the decays' ring: more than the stages of the tiles' plus two chunks
 constexpr int MAX_STAGES = 5;
@@ -72,6 +75,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -158,10 +163,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 __device__ __forceinline__ float2 as_float2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
-// Bounded waits, with the loop out of line: the roles' loops have to fit the instruction caches together.  A wait that runs out sets
-// the abort flag, and every wait of the CTA then returns at once: the roles run through what is left, on whatever they find.
-__device__ __noinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    mbar_wait(bar, parity, abort_flag, status);
+// Bounded waits in few instructions: the roles' loops have to fit the instruction caches together.  A wait that runs out sets the
+// abort flag, and every wait of the CTA then returns at once: the roles run through what is left, on whatever they find.
+__device__ __forceinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!mbar_try_wait_parked(bar, parity, 20000u)) {
+        if (*abort_flag) return;
+        if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
+            *abort_flag = 1;
+            atomicExch(status, (int)DEV_TIMEOUT);
+            return;
+        }
+    }
 }
 struct Waits {
     volatile int *abort_flag;
@@ -229,7 +243,7 @@ __device__ __forceinline__ Work work_of(const ChunkParams &p) {
 
 // The recurrence as it is written, for a CTA's tokens: thread = column of the state, which lies in shared memory.
 template <bool STATES_ONLY>
-__device__ __noinline__ void recurrence(const ChunkParams &p, const Work &w, float *S) {
+__device__ __forceinline__ void recurrence(const ChunkParams &p, const Work &w, float *S) {
     const int c = threadIdx.x;
     if (c >= p.a.dv) return;
     const LinAttnParams &a = p.a;
@@ -261,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     constexpr int KH = DK / 64;                         // half tiles of a key or query tile
     constexpr int STAGE = (2 * KH + 2) * HALF_TILE;     // K, Q, V
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023);     // (an offset, so that accesses stay those of shared memory)
     const int stages = p.stages;
     uint8_t *P = smem + stages * STAGE;                 // [2][64 keys][64 queries] bf16, swizzled like the tiles
     __nv_bfloat16 *O = (__nv_bfloat16 *)(P + 2 * HALF_TILE);        // [64 queries][128], groups of eight values at (group ^ query % 8)
@@ -320,6 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
 
     if (warp < STATE_WARPS) {
         // ------------------------------------------------------------ the state, and V's weighted terms
+        more_registers<STATE_REGS>();
         const int quarter = warp & 3, half = warp >> 2, dv = quarter * 32 + lane;
         const bool rows = quarter * 32 < a.dv, mine = dv < a.dv;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -424,6 +439,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 const int k = half * R + i;
                 if (k < a.dk) w.to[(long long)k * a.dv + dv] = (&S[i / 2].x)[i & 1];
             }
+        fewer_registers<REGS>();
     } else if (warp < LOAD0) {
         // ------------------------------------------------------------ weights of pairs, outputs
         const int quarter = warp - OUT0, t = tid - OUT0 * 32;
@@ -532,197 +548,201 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         }
         tc_fence_before();
         __syncthreads();
-    } else if (warp < DECAY_WARP) {
-        // ------------------------------------------------------------ loads
-        // A thread copies one 16-byte group of every `step`-th row of a tile, 64 / step times.
-        const int t = tid - LOAD0 * 32;
-        const bool all_vec = p.vec[0] && p.vec[1] && p.vec[2];
-        int stage = 0;
-        uint32_t phase = 0;
+    } else {
+        fewer_registers<OTHER_REGS>();
+        if (warp < DECAY_WARP) {
+            // ------------------------------------------------------------ loads
+            // A thread copies one 16-byte group of every `step`-th row of a tile, 64 / step times.
+            const int t = tid - LOAD0 * 32;
+            const bool all_vec = p.vec[0] && p.vec[1] && p.vec[2];
+            int stage = 0;
+            uint32_t phase = 0;
 #pragma unroll 1
-        for (int n = 0; n < N; n++) {
-            if (n >= stages) wait(&empty[stage], phase ^ 1);
-            const int m = min(C, w.n - n * C);
+            for (int n = 0; n < N; n++) {
+                if (n >= stages) wait(&empty[stage], phase ^ 1);
+                const int m = min(C, w.n - n * C);
 #pragma unroll 1
-            for (int which = STATES_ONLY ? 1 : 0; which < 3; which++) {     // q, k, v
-                const TokenView &view = which == 0 ? a.q : which == 1 ? a.k : a.v;
-                const int width = which == 2 ? a.dv : a.dk, per = width > 64 ? 16 : 8, step = 32 * LOAD_WARPS / per;
-                const int c = t & (per - 1), r0 = t / per, bytes = 2 * min(8, width - c * 8);
-                if (bytes <= 0) continue;
-                // the swizzle of row r0 + i * step: that of r0, with its upper bit inverted for the odd ones of steps of four
-                const uint32_t dst = smem_u32(smem + stage * STAGE + (which == 2 ? 2 * KH : which == 0 ? KH : 0) * HALF_TILE + (c >> 3) * HALF_TILE) + r0 * 128;
-                uint32_t d0 = dst + (((c & 7) ^ r0) << 4), d1 = dst + step * 128 + (((c & 7) ^ (r0 + step & 7)) << 4);
-                const long long token = view.token * 2;
-                const char *first = (const char *)view.p + 2 * token_base(a, view, w.b, w.s, which == 2 ? w.h : w.h / a.group) +
-                                    (w.t0 + n * C) * token + c * 16;
-                const char *src = first + r0 * token;
-                if (p.vec[which] && m == C) {
+                for (int which = STATES_ONLY ? 1 : 0; which < 3; which++) {     // q, k, v
+                    const TokenView &view = which == 0 ? a.q : which == 1 ? a.k : a.v;
+                    const int width = which == 2 ? a.dv : a.dk, per = width > 64 ? 16 : 8, step = 32 * LOAD_WARPS / per;
+                    const int c = t & (per - 1), r0 = t / per, bytes = 2 * min(8, width - c * 8);
+                    if (bytes <= 0) continue;
+                    // the swizzle of row r0 + i * step: that of r0, with its upper bit inverted for the odd ones of steps of four
+                    const uint32_t dst = smem_u32(smem + stage * STAGE + (which == 2 ? 2 * KH : which == 0 ? KH : 0) * HALF_TILE + (c >> 3) * HALF_TILE) + r0 * 128;
+                    uint32_t d0 = dst + (((c & 7) ^ r0) << 4), d1 = dst + step * 128 + (((c & 7) ^ (r0 + step & 7)) << 4);
+                    const long long token = view.token * 2;
+                    const char *first = (const char *)view.p + 2 * token_base(a, view, w.b, w.s, which == 2 ? w.h : w.h / a.group) +
+                                        (w.t0 + n * C) * token + c * 16;
+                    const char *src = first + r0 * token;
+                    if (p.vec[which] && m == C) {
 #pragma unroll 1
-                    for (int i = 0; i < per; i += 8) {
+                        for (int i = 0; i < per; i += 8) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            cp_async16(d0, src, bytes);
+                            for (int e = 0; e < 4; e++) {
+                                cp_async16(d0, src, bytes);
+                                src += step * token;
+                                cp_async16(d1, src, bytes);
+                                src += step * token;
+                                d0 += step * 256;
+                                d1 += step * 256;
+                            }
+                        }
+                    } else {                    // of rows past the end nothing is read, zeros arrive
+#pragma unroll 1
+                        for (int r = r0; r < C; r += step) {
+                            if (p.vec[which]) cp_async16(d0, r < m ? src : first, r < m ? bytes : 0);
+                            else copy_values(d0, (const __nv_bfloat16 *)(r < m ? src : first), r < m ? bytes / 2 : 0);
                             src += step * token;
-                            cp_async16(d1, src, bytes);
-                            src += step * token;
-                            d0 += step * 256;
-                            d1 += step * 256;
+                            const uint32_t next = d0 + step * 256;
+                            d0 = d1;
+                            d1 = next;
                         }
                     }
-                } else {                    // of rows past the end nothing is read, zeros arrive
-#pragma unroll 1
-                    for (int r = r0; r < C; r += step) {
-                        if (p.vec[which]) cp_async16(d0, r < m ? src : first, r < m ? bytes : 0);
-                        else copy_values(d0, (const __nv_bfloat16 *)(r < m ? src : first), r < m ? bytes / 2 : 0);
-                        src += step * token;
-                        const uint32_t next = d0 + step * 256;
-                        d0 = d1;
-                        d1 = next;
-                    }
                 }
+                if (all_vec) {
+                    cp_async_arrive(&full[stage]);
+                } else {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    mbar_arrive(&full[stage]);
+                }
+                if (++stage == stages) stage = 0, phase ^= 1;
             }
-            if (all_vec) {
-                cp_async_arrive(&full[stage]);
-            } else {
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                mbar_arrive(&full[stage]);
-            }
-            if (++stage == stages) stage = 0, phase ^= 1;
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        tc_fence_before();
-        __syncthreads();
-    } else if (warp == DECAY_WARP) {
-        // ------------------------------------------------------------ decays
-        const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
-        int stage = 0;
-        uint32_t phase = 0;
-        float total = 0.0f;
-        bool any = false;
-        float2 next = make_float2(0.0f, 0.0f);
-        auto decays = [&](int n) {              // of tokens 2 * lane and the one behind it, 0 past the end
-            const int i = n * C + 2 * lane;
-            float2 f = make_float2(0.0f, 0.0f);
-            if (g && i < w.n) f.x = g[(w.t0 + i) * a.g.token];
-            if (g && i + 1 < w.n) f.y = g[(w.t0 + i + 1) * a.g.token];
-            return f;
-        };
-        if (N > 0) next = decays(0);
-        for (int n = 0; n < N; n++) {
-            if (n >= stages) wait(&empty[stage], phase ^ 1);
-            const float2 f = next;
-            if (n + 1 < N) next = decays(n + 1);
-            Decays &d = dec[n % SLOTS];
-            const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
-            const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
-            float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
-                if (lane >= o) up += u;
-                if (lane + o < 32) down += v2;
-            }
-            const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1);
-            float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-            if (lane == 0) before = 0.0f;
-            if (lane == 31) behind = 0.0f;
-            const unsigned upto = 0xffffffffu >> (31 - lane), under = upto >> 1;        // lanes up to this one; below it
-            const bool reset_before = ((even | odds) & under) != 0, reset_behind = ((even | odds) & ~upto) != 0;
-            const float s0 = before + g0;
-            constexpr float LOG2E = 1.4426950408889634f;
-            *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0 * LOG2E, up * LOG2E);
-            *(float2 *)(d.from_start + 2 * lane) =
-                make_float2(reset_before || r0 ? 0.0f : p.scale * expf(s0), reset_before || r0 || r1 ? 0.0f : p.scale * expf(up));
-            *(float2 *)(d.to_end + 2 * lane) = make_float2(reset_behind || r1 ? 0.0f : expf(behind + g1), reset_behind ? 0.0f : expf(behind));
-            // a bit per token from a bit per pair
-            unsigned long long bits = 0;
-            if ((even | odds) != 0 && lane == 0)
-#pragma unroll 1
-                for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
-            const float sum = __shfl_sync(0xffffffffu, up, 31);
-            if (lane == 0) {
-                d.resets[0] = (unsigned)bits;
-                d.resets[1] = (unsigned)(bits >> 32);
-                d.less = (even | odds) ? -1.0f : expm1f(sum);
-            }
-            total += sum;
-            any = any || (even | odds) != 0;
-            mbar_arrive(&full[stage]);
-            if (++stage == stages) stage = 0, phase ^= 1;
-        }
-        if (STATES_ONLY && lane == 0 && served)
-            p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
-        tc_fence_before();
-        __syncthreads();
-    } else {
-        // ------------------------------------------------------------ MMAs, by one thread
-        if (lane == 0 && N > 0) {
-            int stage = 0, next_stage = 0;
-            uint32_t next_phase = 0;
-            const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0;
-            const uint32_t negative = p.negative << 13;         // of A: a negative scale
-            auto wait1 = [&](uint64_t *bar, uint32_t parity) {
-                if (!mbar_try_wait(bar, parity)) wait_long(smem_u32(bar), parity, abort_flag, p.status);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            tc_fence_before();
+            __syncthreads();
+        } else if (warp == DECAY_WARP) {
+            // ------------------------------------------------------------ decays
+            const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
+            int stage = 0;
+            uint32_t phase = 0;
+            float total = 0.0f;
+            bool any = false;
+            float2 next = make_float2(0.0f, 0.0f);
+            auto decays = [&](int n) {              // of tokens 2 * lane and the one behind it, 0 past the end
+                const int i = n * C + 2 * lane;
+                float2 f = make_float2(0.0f, 0.0f);
+                if (g && i < w.n) f.x = g[(w.t0 + i) * a.g.token];
+                if (g && i + 1 < w.n) f.y = g[(w.t0 + i + 1) * a.g.token];
+                return f;
             };
-#pragma unroll 1
-            for (int n = -1; n < N; n++) {
-                const uint32_t k = smem_u32(smem + stage * STAGE), q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
-                if (n >= 0) {
-                    wait1(v_full, n & 1);
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int term = 2; term >= 0; term--)
+            if (N > 0) next = decays(0);
+            for (int n = 0; n < N; n++) {
+                if (n >= stages) wait(&empty[stage], phase ^ 1);
+                const float2 f = next;
+                if (n + 1 < N) next = decays(n + 1);
+                Decays &d = dec[n % SLOTS];
+                const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
+                const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
+                float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
 #pragma unroll
-                        for (int i = 0; i < C / 16; i++)
-                            umma_bf16_ts(tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
-                                         idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
-                    umma_commit(d_full);
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
+                    if (lane >= o) up += u;
+                    if (lane + o < 32) down += v2;
                 }
-                if (n + 1 < N) {
-                    // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
-                    wait1(&full[next_stage], next_phase);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    if (!STATES_ONLY) {
-                        if (n >= 0) wait1(kq_empty, n & 1);
+                const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1);
+                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+                if (lane == 0) before = 0.0f;
+                if (lane == 31) behind = 0.0f;
+                const unsigned upto = 0xffffffffu >> (31 - lane), under = upto >> 1;        // lanes up to this one; below it
+                const bool reset_before = ((even | odds) & under) != 0, reset_behind = ((even | odds) & ~upto) != 0;
+                const float s0 = before + g0;
+                constexpr float LOG2E = 1.4426950408889634f;
+                *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0 * LOG2E, up * LOG2E);
+                *(float2 *)(d.from_start + 2 * lane) =
+                    make_float2(reset_before || r0 ? 0.0f : p.scale * expf(s0), reset_before || r0 || r1 ? 0.0f : p.scale * expf(up));
+                *(float2 *)(d.to_end + 2 * lane) = make_float2(reset_behind || r1 ? 0.0f : expf(behind + g1), reset_behind ? 0.0f : expf(behind));
+                // a bit per token from a bit per pair
+                unsigned long long bits = 0;
+                if ((even | odds) != 0 && lane == 0)
+#pragma unroll 1
+                    for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
+                const float sum = __shfl_sync(0xffffffffu, up, 31);
+                if (lane == 0) {
+                    d.resets[0] = (unsigned)bits;
+                    d.resets[1] = (unsigned)(bits >> 32);
+                    d.less = (even | odds) ? -1.0f : expm1f(sum);
+                }
+                total += sum;
+                any = any || (even | odds) != 0;
+                mbar_arrive(&full[stage]);
+                if (++stage == stages) stage = 0, phase ^= 1;
+            }
+            if (STATES_ONLY && lane == 0 && served)
+                p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
+            tc_fence_before();
+            __syncthreads();
+        } else {
+            // ------------------------------------------------------------ MMAs, by one thread
+            if (lane == 0 && N > 0) {
+                int stage = 0, next_stage = 0;
+                uint32_t next_phase = 0;
+                const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0;
+                const uint32_t negative = p.negative << 13;         // of A: a negative scale
+                auto wait1 = [&](uint64_t *bar, uint32_t parity) {
+                    if (!mbar_try_wait(bar, parity)) wait_long(smem_u32(bar), parity, abort_flag, p.status);
+                };
+#pragma unroll 1
+                for (int n = -1; n < N; n++) {
+                    const uint32_t k = smem_u32(smem + stage * STAGE), q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
+                    if (n >= 0) {
+                        wait1(v_full, n & 1);
                         tc_fence_after();
-                        const uint32_t k1 = smem_u32(smem + next_stage * STAGE);
+#pragma unroll 1
+                        for (int term = 2; term >= 0; term--)
+#pragma unroll
+                            for (int i = 0; i < C / 16; i++)
+                                umma_bf16_ts(tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
+                                             idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
+                        umma_commit(d_full);
+                    }
+                    if (n + 1 < N) {
+                        // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
+                        wait1(&full[next_stage], next_phase);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        if (!STATES_ONLY) {
+                            if (n >= 0) wait1(kq_empty, n & 1);
+                            tc_fence_after();
+                            const uint32_t k1 = smem_u32(smem + next_stage * STAGE);
+#pragma unroll 1
+                            for (int h = 0; h < KH; h++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    umma_bf16(tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
+                                              idesc_bf16(64, C, 0, 0), (h | i) != 0);
+                            umma_commit(kq_full);
+                        }
+                        if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
+                    }
+                    if (n < 0) continue;
+                    if (!STATES_ONLY) {
+                        wait1(s_full, n & 1);
+                        if (n > 0) wait1(o_empty, (n - 1) & 1);
+                        tc_fence_after();
 #pragma unroll 1
                         for (int h = 0; h < KH; h++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                umma_bf16(tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
-                                          idesc_bf16(64, C, 0, 0), (h | i) != 0);
-                        umma_commit(kq_full);
+                                umma_bf16_ts(tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
+                                             idesc_bf16(128, C, 0, 0), (h | i) != 0);
+                        umma_commit(s_empty);
+                        wait1(&p_full[n & 1], n >> 1 & 1);
+                        const uint32_t pt = smem_u32(P + (n & 1) * HALF_TILE);
+#pragma unroll
+                        for (int i = 0; i < C / 16; i++)
+                            umma_bf16(tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE),
+                                      idesc_bf16(128, C, 1, 1) | negative, i != 0);
+                        umma_commit(o_full);
                     }
-                    if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
+                    umma_commit(&empty[stage]);
+                    if (++stage == stages) stage = 0;
                 }
-                if (n < 0) continue;
-                if (!STATES_ONLY) {
-                    wait1(s_full, n & 1);
-                    if (n > 0) wait1(o_empty, (n - 1) & 1);
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int h = 0; h < KH; h++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            umma_bf16_ts(tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
-                                         idesc_bf16(128, C, 0, 0), (h | i) != 0);
-                    umma_commit(s_empty);
-                    wait1(&p_full[n & 1], n >> 1 & 1);
-                    const uint32_t pt = smem_u32(P + (n & 1) * HALF_TILE);
-#pragma unroll
-                    for (int i = 0; i < C / 16; i++)
-                        umma_bf16(tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE),
-                                  idesc_bf16(128, C, 1, 1) | negative, i != 0);
-                    umma_commit(o_full);
-                }
-                umma_commit(&empty[stage]);
-                if (++stage == stages) stage = 0;
             }
+            __syncwarp();
+            tc_fence_before();
+            __syncthreads();
         }
-        __syncwarp();
-        tc_fence_before();
-        __syncthreads();
+        more_registers<REGS>();
     }
 
     // ---------------------------------------------------------------- teardown (every warp has passed the barrier above)
@@ -771,6 +791,10 @@ void launch_chunks(nb_handle_s *h, const ChunkParams &p) {
     auto kernel = linear_attention_chunk_kernel<DK, STATES_ONLY>;
     const unsigned bit = 1u << (DK / 64 - 1 + (STATES_ONLY ? 2 : 0));
     if (!(h->linear_attention_ready & bit)) {
+        cudaFuncAttributes fa;
+        NB_CHECK_CUDA(cudaFuncGetAttributes(&fa, kernel));
+        // the warpgroups' requests add up to what REGS registers a thread make; fewer, and they would wait for good
+        if (fa.numRegs != REGS) throw Error(NB_ERR_UNSUPPORTED, "linear attention: the kernel was compiled with another number of registers");
         NB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<DK>()));
         h->linear_attention_ready |= bit;
     }
