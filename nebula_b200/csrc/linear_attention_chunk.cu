@@ -33,12 +33,16 @@ using namespace tc;
 namespace {
 
 constexpr int C = 64;                       // tokens of a chunk
-constexpr int STATE_WARPS = 8, OUT_WARPS = 4, LOAD_WARPS = 2;
-constexpr int OUT0 = STATE_WARPS, LOAD0 = OUT0 + OUT_WARPS, DECAY_WARP = LOAD0 + LOAD_WARPS, MMA_WARP = DECAY_WARP + 1;
+// Roles by warpgroup: two for the state, two for V's weighted terms, one each for the weights of pairs and for the outputs; then a
+// warp of loads for each of Q (and the decays), K and V, and the one that issues MMAs.  Many warps of few registers: what they do is a chain of short
+// steps, and with four warps to a scheduler (state and terms in one role, weights and outputs in another) a chunk took 4300 cycles.
+constexpr int STATE_WARPS = 8, TERM_WARPS = 8, PAIR_WARPS = 4, OUT_WARPS = 4, LOAD_WARPS = 3;
+constexpr int TERM0 = STATE_WARPS, PAIR0 = TERM0 + TERM_WARPS, OUT0 = PAIR0 + PAIR_WARPS, LOAD0 = OUT0 + OUT_WARPS;
+constexpr int MMA_WARP = LOAD0 + LOAD_WARPS;
 constexpr int THREADS = 32 * (MMA_WARP + 1);
-// Registers of a thread: what a launch of so many threads gets, and how the warpgroups share it (their sum is at most four times that)
-constexpr int REGS = 128, STATE_REGS = 160, OUT_REGS = 128, OTHER_REGS = 64;
-static_assert(THREADS == 512 && 2 * STATE_REGS + OUT_REGS + OTHER_REGS <= 4 * REGS, "registers");
+// Registers of a thread: what a launch of so many threads gets, and how the warpgroups share it (their sum is at most seven times that)
+constexpr int REGS = 72, STATE_REGS = 104, TERM_REGS = 64, PAIR_REGS = 56, OUT_REGS = 56, OTHER_REGS = 56;
+static_assert(THREADS == 896 && 2 * STATE_REGS + 2 * TERM_REGS + PAIR_REGS + OUT_REGS + OTHER_REGS <= 7 * REGS, "registers");
 constexpr int HALF_TILE = C * 128;          // [64 tokens][64 values] of bf16, rows of 128 bytes, 128-byte swizzle
 constexpr int SLOTS = 8;                    // of the decays' ring: more than the stages of the tiles' plus two chunks
 constexpr int MAX_STAGES = 5;
@@ -87,15 +91,21 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, int a_mn, int b_
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void umma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Issued by the lane with `leader`; the whole warp passes, so that the operands stay in uniform registers.
+__device__ __forceinline__ void umma_bf16(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_bf16_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void umma_done(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader) : "memory");
 }
 // Shared-memory descriptor with 128-byte swizzle and groups of eight rows 1024 bytes apart.  K-major operands: eight M/N rows a
 // group.  M/N-major ones: eight K rows a group, and `mn_step` bytes to the next 64 M/N values.
@@ -112,16 +122,19 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t *v)
 }
 // 16 lanes of tensor memory in the layout of matrix fragments: thread t holds rows t / 4 and t / 4 + 8.  Loads: of every eight columns
 // 2 (t % 4) and the next one, of both rows; stores of four columns: column t % 4, of both rows.
-__device__ __forceinline__ void tmem_ld_16x256_x8(uint32_t taddr, uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t (&v)[8]) {
+    __syncwarp();
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t (&v)[16]) {
     __syncwarp();
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr)
         : "memory");
 }
@@ -166,11 +179,11 @@ __device__ __forceinline__ float2 as_float2(uint32_t a, uint32_t b) { return mak
 // Bounded waits in few instructions: the roles' loops have to fit the instruction caches together.  A wait that runs out sets the
 // abort flag, and every wait of the CTA then returns at once: the roles run through what is left, on whatever they find.
 __device__ __forceinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    const long long t0 = clock64();
+    const unsigned t0 = (unsigned)clock();
 #pragma unroll 1
     while (!mbar_try_wait_parked(bar, parity, 20000u)) {
         if (*abort_flag) return;
-        if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
+        if ((unsigned)clock() - t0 > (unsigned)WAIT_LIMIT_CYCLES) {
             *abort_flag = 1;
             atomicExch(status, (int)DEV_TIMEOUT);
             return;
@@ -283,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     uint64_t *bars = (uint64_t *)(dec + SLOTS);
     uint64_t *full = bars, *empty = bars + MAX_STAGES;  // loaders -> all, MMA -> loaders
     uint64_t *kq_full = empty + MAX_STAGES, *kq_empty = kq_full + 1, *p_full = kq_empty + 1 /* [2] */, *o_full = p_full + 2, *o_empty = o_full + 1;
-    uint64_t *v_full = o_empty + 1, *d_full = v_full + 1, *s_full = d_full + 1, *s_empty = s_full + 1;
+    uint64_t *v_full = o_empty + 1, *d_empty = v_full + 1, *d_full = d_empty + 1, *s_full = d_full + 1, *s_empty = s_full + 1;
     uint32_t *tmem_slot = (uint32_t *)(s_empty + 1);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     int *odd = (int *)(tmem_slot + 2);                  // infinities or NaN were met
@@ -292,16 +305,17 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     grid_dependents_start();
     if (tid == 0) {
         for (int s = 0; s < MAX_STAGES; s++) {
-            mbar_init(&full[s], 32 * LOAD_WARPS + 32);
+            mbar_init(&full[s], 32 * (STATES_ONLY ? 2 : 3) + 32);      // a copy from each lane of the loading warps, and the decays
             mbar_init(&empty[s], 1);
         }
         mbar_init(kq_full, 1);
-        mbar_init(kq_empty, OUT_WARPS);
-        mbar_init(&p_full[0], OUT_WARPS);
-        mbar_init(&p_full[1], OUT_WARPS);
+        mbar_init(kq_empty, PAIR_WARPS);
+        mbar_init(&p_full[0], PAIR_WARPS);
+        mbar_init(&p_full[1], PAIR_WARPS);
         mbar_init(o_full, 1);
         mbar_init(o_empty, OUT_WARPS);
-        mbar_init(v_full, STATE_WARPS);
+        mbar_init(v_full, TERM_WARPS);
+        mbar_init(d_empty, STATE_WARPS);
         mbar_init(d_full, 1);
         mbar_init(s_full, STATE_WARPS);
         mbar_init(s_empty, 1);
@@ -333,98 +347,59 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     const Waits wait = {abort_flag, p.status};
 
     if (warp < STATE_WARPS) {
-        // ------------------------------------------------------------ the state, and V's weighted terms
+        // ------------------------------------------------------------ the state
         more_registers<STATE_REGS>();
         const int quarter = warp & 3, half = warp >> 2, dv = quarter * 32 + lane;
-        const bool rows = quarter * 32 < a.dv, mine = dv < a.dv;
+        const bool mine = dv < a.dv;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
         constexpr int R = DK / 2;                       // columns of the state of a thread: keys half * R ...
+        const int keys = mine ? min(max(a.dk - half * R, 0), R) : 0;
         float2 S[R / 2];
+        {
+            const float *from = served && w.from ? w.from + (long long)half * R * a.dv + dv : nullptr;
+            const int n = from ? keys : 0;
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            const int k = half * R + i;
-            (&S[i / 2].x)[i & 1] = served && w.from && mine && k < a.dk ? w.from[(long long)k * a.dv + dv] : 0.0f;
+            for (int i = 0; i < R; i++) {
+                (&S[i / 2].x)[i & 1] = i < n ? *from : 0.0f;
+                from += a.dv;
+            }
         }
-        // V [dv][token] of half of the chunk's tokens, in pairs of tokens and in the layout of fragments: [16 dv][8 tokens][dv, dv + 8]
-        uint32_t v[16];
-        float2 by[4];
-        int stage = 0;
-        uint32_t phase = 0;
-        const uint32_t v_at = smem_u32(smem) + 2 * KH * HALF_TILE + (quarter >> 1) * HALF_TILE + (half * 32 + (lane >> 4) * 8 + (lane & 7)) * 128;
-        // chunk n's state while chunk n + 1's values are prepared
 #pragma unroll 1
-        for (int n = -1; n < N; n++) {
-            const bool more = n + 1 < N;
-            if (more) {
-                wait(&full[stage], phase);
-                if (rows) {
-                    const uint32_t tile = v_at + stage * STAGE;
+        for (int n = 0; n < N; n++) {
+            if (!STATES_ONLY) {                         // what the queries read
+                wait(s_empty, (n - 1) & 1);             // (at first: at once)
+                tc_fence_after();
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t group = ((((quarter & 1) * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
-                        ldmatrix_trans(tile + group, v + h * 8);
-                        ldmatrix_trans(tile + group + 16 * 128, v + h * 8 + 4);
-                    }
+                for (int c = 0; c < R / 2; c += 16) {
+                    uint32_t x[16];
 #pragma unroll
-                    for (int t = 0; t < 4; t++) by[t] = *(const float2 *)(dec[(n + 1) % SLOTS].to_end + half * 32 + t * 8 + (lane & 3) * 2);
+                    for (int i = 0; i < 16; i++) x[i] = pack_bf16(S[c + i].x, S[c + i].y);
+                    tmem_st_32x16(at + T_S + half * (R / 2) + c, x);
                 }
-                if (++stage == stages) stage = 0, phase ^= 1;
-            }
-            if (n >= 0) wait(d_full, n & 1);
-            tc_fence_after();
-            if (more && rows) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float2 x[8];
-                    uint32_t y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = mul2(make_float2(low_value(v[h * 8 + i]), high_value(v[h * 8 + i])), by[i / 2]);
-#pragma unroll
-                    for (int term = 0; term < 3; term++) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            y[i] = pack_high(x[i].x, x[i].y);
-                            if (term < 2) x[i] = fma2(make_float2(-1.0f, -1.0f), make_float2(high_part(x[i].x), high_part(x[i].y)), x[i]);
-                        }
-                        tmem_st_16x128_x4(at + ((uint32_t)(h * 16) << 16) + T_VW + term * 32 + half * 16, y);
-                    }
-                }
-            }
-            if (n >= 0) {
-                const float less = dec[n % SLOTS].less;
-#pragma unroll
-                for (int c = 0; c < R; c += 32) {
-                    uint32_t d[32];
-                    tmem_ld_32x32(at + T_D + half * R + c, d);
-                    tmem_ld_wait();
-                    // as S + (less S + new): what a decay near 1 takes away keeps its own precision.  Once a value is not finite it
-                    // stays so, whatever the decays
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        float2 &x = S[c / 2 + i];
-                        x = add2(x, fma2(make_float2(less, less), x, make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]))));
-                    }
-                }
-            }
-            if (more) {
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(v_full);
-                if (!STATES_ONLY) {
-                    uint32_t x[R / 2];
+                if (lane == 0) mbar_arrive(s_full);
+            }
+            wait(d_full, n & 1);
+            tc_fence_after();
+            const float less = dec[n % SLOTS].less;
 #pragma unroll
-                    for (int i = 0; i < R / 2; i++) x[i] = pack_bf16(S[i].x, S[i].y);
-                    if (n >= 0) wait(s_empty, n & 1);
-                    tc_fence_after();
-                    if constexpr (R == 64) tmem_st_32x32(at + T_S + half * 32, x);
-                    else tmem_st_32x16(at + T_S + half * 16, x);
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(s_full);
+            for (int c = 0; c < R; c += 16) {
+                uint32_t d[16];
+                tmem_ld_32x16(at + T_D + half * R + c, d);
+                tmem_ld_wait();
+                // as S + (less S + new): what a decay near 1 takes away keeps its own precision.  Once a value is not finite it
+                // stays so, whatever the decays
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float2 &x = S[c / 2 + i];
+                    x = add2(x, fma2(make_float2(less, less), x, as_float2(d[2 * i], d[2 * i + 1])));
                 }
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(d_empty);
         }
         // infinities and NaN, of the first state, keys or values, are in the last state whatever the decays were
         float bad = 0.0f;
@@ -433,16 +408,123 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         if (mine && bad != 0.0f) *odd = 1;
         tc_fence_before();
         __syncthreads();
-        if (served && w.to && mine && !*odd && !*abort_flag)
+        if (served && w.to && !*odd && !*abort_flag) {
+            float *to = w.to + (long long)half * R * a.dv + dv;
 #pragma unroll
             for (int i = 0; i < R; i++) {
-                const int k = half * R + i;
-                if (k < a.dk) w.to[(long long)k * a.dv + dv] = (&S[i / 2].x)[i & 1];
+                if (i < keys) *to = (&S[i / 2].x)[i & 1];
+                to += a.dv;
             }
+        }
         fewer_registers<REGS>();
+    } else if (warp < PAIR0) {
+        // ------------------------------------------------------------ V's weighted terms
+        fewer_registers<TERM_REGS>();
+        const int quarter = warp & 3, half = (warp - TERM0) >> 2;       // 32 values of the head, 32 tokens of the chunk
+        const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + T_VW + half * 16;
+        // V [dv][token] in pairs of tokens and in the layout of fragments: [16 dv][8 tokens][dv, dv + 8]
+        const uint32_t v_at = smem_u32(smem) + 2 * KH * HALF_TILE + (quarter >> 1) * HALF_TILE + (half * 32 + (lane >> 4) * 8 + (lane & 7)) * 128;
+        int stage = 0;
+        uint32_t phase = 0;
+#pragma unroll 1
+        for (int n = 0; n < N; n++) {
+            wait(&full[stage], phase);
+            if (quarter * 32 < a.dv) {
+                const uint32_t tile = v_at + stage * STAGE;
+                float2 by[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) by[t] = *(const float2 *)(dec[n % SLOTS].to_end + half * 32 + t * 8 + (lane & 3) * 2);
+#pragma unroll 1
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t group = tile + ((((quarter & 1) * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
+                    uint32_t v[8];
+                    ldmatrix_trans(group, v);
+                    ldmatrix_trans(group + 16 * 128, v + 4);
+                    float2 x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = mul2(make_float2(low_value(v[i]), high_value(v[i])), by[i / 2]);
+                    if (h == 0) wait(d_full, (n - 1) & 1);          // the terms in tensor memory have been read (at first: at once)
+                    tc_fence_after();
+#pragma unroll
+                    for (int term = 0; term < 3; term++) {
+                        uint32_t y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            y[i] = pack_high(x[i].x, x[i].y);
+                            if (term < 2) x[i] = fma2(make_float2(-1.0f, -1.0f), make_float2(high_part(x[i].x), high_part(x[i].y)), x[i]);
+                        }
+                        tmem_st_16x128_x4(at + ((uint32_t)(h * 16) << 16) + term * 32, y);
+                    }
+                }
+                tmem_st_wait();
+            } else {
+                wait(d_full, (n - 1) & 1);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_full);
+            if (++stage == stages) stage = 0, phase ^= 1;
+        }
+        tc_fence_before();
+        __syncthreads();
+        more_registers<REGS>();
+    } else if (warp < OUT0) {
+        // ------------------------------------------------------------ weights of pairs
+        fewer_registers<PAIR_REGS>();
+        if (!STATES_ONLY) {
+            const int quarter = warp & 3;
+            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + T_KQ + quarter * 16;
+            int stage = 0;
+            uint32_t phase = 0;
+            // keys r and r + 8 of the 16 of this warp, against the queries from its first key on: 8 g + i1 and the next one
+            const int r = lane >> 2, i1 = 2 * (lane & 3);
+            const uint32_t causal = (i1 >= r ? 0xffffu : 0u) | (i1 + 1 >= r ? 0xffff0000u : 0u);       // of eight of both on the diagonal
+#pragma unroll 1
+            for (int n = 0; n < N; n++) {
+                wait(&full[stage], phase);
+                if (++stage == stages) stage = 0, phase ^= 1;
+                const Decays &d = dec[n % SLOTS];
+                const float m0 = p.log2_size - d.sum2[quarter * 16 + r], m1 = p.log2_size - d.sum2[quarter * 16 + r + 8];
+                const uint32_t row = smem_u32(P) + (n & 1) * HALF_TILE + (quarter * 16 + (lane & 15)) * 128;
+                wait(kq_full, n & 1);
+                tc_fence_after();
+                uint32_t on = causal, above = 0;            // of the keys' own 16 queries: the last eight keys do not see the first eight
+#pragma unroll 1
+                for (int g = 0; g < 8 - 2 * quarter; g += 2) {
+                    uint32_t x[8];
+                    tmem_ld_16x256_x2(at + g * 8, x);
+                    const float2 s = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + i1), t = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + 8 + i1);
+                    const float e[8] = {ex2(s.x + m0), ex2(s.y + m0), ex2(s.x + m1), ex2(s.y + m1), ex2(t.x + m0), ex2(t.y + m0), ex2(t.x + m1), ex2(t.y + m1)};
+                    tmem_ld_wait();
+                    uint32_t y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[i] = pack_bf16(__uint_as_float(x[2 * i]) * e[2 * i], __uint_as_float(x[2 * i + 1]) * e[2 * i + 1]);
+                    stmatrix(row + (((quarter * 2 + g + (lane >> 4)) ^ (lane & 7)) << 4), y[0] & on, y[1] & above, y[2], y[3] & on);
+                    on = above = 0xffffffffu;
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(kq_empty);
+                if (d.resets[0] | d.resets[1]) {        // a key is not seen from the next reset behind it on
+                    __syncwarp();
+                    const int j = quarter * 16 + (lane & 15);
+                    const unsigned long long later = ((unsigned long long)d.resets[1] << 32 | d.resets[0]) & (~0ULL << j << 1);
+#pragma unroll 1
+                    for (int i = later ? __ffsll((long long)later) - 1 + (lane >> 4) : C; i < C; i += 2)
+                        *(__nv_bfloat16 *)(P + (n & 1) * HALF_TILE + j * 128 + (((i >> 3) ^ (j & 7)) << 4) + (i & 7) * 2) = from_f32<__nv_bfloat16>(0.0f);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[n & 1]);
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+        more_registers<REGS>();
     } else if (warp < LOAD0) {
-        // ------------------------------------------------------------ weights of pairs, outputs
-        const int quarter = warp - OUT0, t = tid - OUT0 * 32;
+        // ------------------------------------------------------------ outputs
+        fewer_registers<OUT_REGS>();
+        const int quarter = warp & 3, t = tid - OUT0 * 32;
         __nv_bfloat16 *out = (__nv_bfloat16 *)a.out.p + token_base(a, a.out, w.b, w.s, w.h);
         if (!STATES_ONLY && w.s.slot < 0 && !w.skip)        // not served: zeros
             for (int i = 0; i < w.n; i++)
@@ -450,70 +532,25 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 for (int c = t; c < a.dv; c += 32 * OUT_WARPS) out[(w.t0 + i) * a.out.token + c] = from_f32<__nv_bfloat16>(0.0f);
         if (!STATES_ONLY) {
             const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
-            int stage = 0;
-            uint32_t phase = 0;
-            // of a pair's 16 x 16 tokens on the diagonal: queries 2 (lane % 4) and the next one against key lane / 4, of the same eight
-            const int r = lane >> 2, i1 = 2 * (lane & 3);
-            const uint32_t causal = (i1 >= r ? 0xffffu : 0u) | (i1 + 1 >= r ? 0xffff0000u : 0u);
-            // chunk n's weights of pairs, then chunk n - 1's outputs
 #pragma unroll 1
-            for (int n = 0; n <= N; n++) {
-                if (n < N) {
-                    wait(&full[stage], phase);
-                    if (++stage == stages) stage = 0, phase ^= 1;
-                    wait(kq_full, n & 1);
-                    tc_fence_after();
-                    // keys r and r + 8 of the 16 of this warp, against the queries from its first key on: 8 g + i1 and the next one
-                    // (columns past the last query are not used)
-                    uint32_t x[32];
-                    tmem_ld_16x256_x8(at + T_KQ + quarter * 16, x);
-                    const Decays &d = dec[n % SLOTS];
-                    const float m0 = p.log2_size - d.sum2[quarter * 16 + r], m1 = p.log2_size - d.sum2[quarter * 16 + r + 8];
-                    const uint32_t row = smem_u32(P) + (n & 1) * HALF_TILE + (quarter * 16 + (lane & 15)) * 128;
-                    tmem_ld_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(kq_empty);
-#pragma unroll
-                    for (int g = 0; g < 8; g++) {
-                        if (g % 2 == 0 && g >= 8 - 2 * quarter) break;
-                        const float2 s = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + i1);
-                        x[4 * g] = pack_bf16(__uint_as_float(x[4 * g]) * ex2(s.x + m0), __uint_as_float(x[4 * g + 1]) * ex2(s.y + m0));
-                        x[4 * g + 1] = pack_bf16(__uint_as_float(x[4 * g + 2]) * ex2(s.x + m1), __uint_as_float(x[4 * g + 3]) * ex2(s.y + m1));
-                        if (g == 0) x[0] &= causal, x[1] = 0;
-                        if (g == 1) x[5] &= causal;
-                        if (g & 1)
-                            stmatrix(row + (((quarter * 2 + g - 1 + (lane >> 4)) ^ (lane & 7)) << 4), x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
-                    }
-                    if (d.resets[0] | d.resets[1]) {        // a key is not seen from the next reset behind it on
-                        __syncwarp();
-                        const int j = quarter * 16 + (lane & 15);
-                        const unsigned long long later = ((unsigned long long)d.resets[1] << 32 | d.resets[0]) & (~0ULL << j << 1);
-#pragma unroll 1
-                        for (int i = later ? __ffsll((long long)later) - 1 + (lane >> 4) : C; i < C; i += 2)
-                            *(__nv_bfloat16 *)(P + (n & 1) * HALF_TILE + j * 128 + (((i >> 3) ^ (j & 7)) << 4) + (i & 7) * 2) = from_f32<__nv_bfloat16>(0.0f);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[n & 1]);
-                }
-                if (n == 0) continue;
-                const int before = n - 1;
-                wait(o_full, before & 1);
+            for (int n = 0; n < N; n++) {
+                wait(o_full, n & 1);
                 epilogue_bar_sync(1);                       // the outputs of the chunk before have left shared memory
                 tc_fence_after();
                 if (quarter * 32 < a.dv) {
-                    const float *weight = dec[before % SLOTS].from_start + i1;
+                    const float *weight = dec[n % SLOTS].from_start + 2 * (lane & 3);
 #pragma unroll 1
-                    for (int h = 0; h < 2; h++) {       // 16 values of the head
-                        const uint32_t to = smem_u32(O) + ((lane >> 4) * 8 + (lane & 7)) * 256 + (((quarter * 4 + h * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
-                        uint32_t x[32], y[32];
-                        tmem_ld_16x256_x8(at + ((uint32_t)(h * 16) << 16) + T_O2, x);
-                        tmem_ld_16x256_x8(at + ((uint32_t)(h * 16) << 16) + T_O1, y);
+                    for (int h = 0; h < 4; h++) {       // 16 values of the head, 32 tokens
+                        const uint32_t to = smem_u32(O) + ((h & 1) * 32 + (lane >> 4) * 8 + (lane & 7)) * 256 +
+                                            (((quarter * 4 + (h & 2) + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
+                        const uint32_t from = at + ((uint32_t)((h & 2) * 8) << 16) + (h & 1) * 32;
+                        uint32_t x[16], y[16];
+                        tmem_ld_16x256_x4(from + T_O2, x);
+                        tmem_ld_16x256_x4(from + T_O1, y);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int g = 0; g < 8; g++) {
-                            const float2 e = *(const float2 *)(weight + g * 8);
+                        for (int g = 0; g < 4; g++) {
+                            const float2 e = *(const float2 *)(weight + (h & 1) * 32 + g * 8);
                             const float2 o0 = fma2(e, as_float2(x[4 * g], x[4 * g + 1]), as_float2(y[4 * g], y[4 * g + 1]));
                             const float2 o1 = fma2(e, as_float2(x[4 * g + 2], x[4 * g + 3]), as_float2(y[4 * g + 2], y[4 * g + 3]));
                             x[4 * g] = pack_bf16(o0.x, o0.y);
@@ -526,14 +563,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_empty);
                 epilogue_bar_sync(1);
-                const int t0 = w.t0 + before * C, m = min(C, w.n - before * C);
+                const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
                 if (p.out_vec) {
                     const int c = t & 15;
                     if (c * 8 < a.dv) {
                         const __nv_bfloat16 *from = O + (t >> 4) * 128 + ((c ^ (t >> 4)) << 3);
                         __nv_bfloat16 *to = out + (t0 + (t >> 4)) * a.out.token + c * 8;
                         if (m == C) {
-#pragma unroll
+#pragma unroll 4
                             for (int i = 0; i < 8; i++, to += 8 * a.out.token) *(uint4 *)to = *(const uint4 *)(from + i * 8 * 128);
                         } else {
 #pragma unroll 1
@@ -548,197 +585,187 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         }
         tc_fence_before();
         __syncthreads();
+        more_registers<REGS>();
     } else {
         fewer_registers<OTHER_REGS>();
-        if (warp < DECAY_WARP) {
-            // ------------------------------------------------------------ loads
-            // A thread copies one 16-byte group of every `step`-th row of a tile, 64 / step times.
-            const int t = tid - LOAD0 * 32;
-            const bool all_vec = p.vec[0] && p.vec[1] && p.vec[2];
+        if (warp < MMA_WARP) {
+            // ------------------------------------------------------------ loads, and the decays
+            // A warp copies a tile of one tensor (q, k, v): a lane one 16-byte group of every second row (of four, where rows are of up to
+            // eight groups).
+            const int which = warp - LOAD0;
+            const bool copies = !STATES_ONLY || which != 0;
+            const TokenView &view = which == 0 ? a.q : which == 1 ? a.k : a.v;
+            const int width = which == 2 ? a.dv : a.dk, rows = width > 64 ? 2 : 4;
+            const int c = width > 64 ? lane & 15 : lane & 7, r0 = width > 64 ? lane >> 4 : lane >> 3, bytes = 2 * min(8, width - c * 8);
+            const bool vec = p.vec[which];
+            const long long pitch = view.token * 2, step = rows * pitch;
+            const char *src = (const char *)view.p + 2 * (token_base(a, view, w.b, w.s, which == 2 ? w.h : w.h / a.group) + (w.t0 + r0) * view.token) + c * 16;
+            const uint32_t dst = smem_u32(smem) + (which == 0 ? KH : which == 1 ? 0 : 2 * KH) * HALF_TILE + (c >> 3) * HALF_TILE + r0 * 128 + (((c & 7) ^ r0) << 4);
+            // what the swizzle of the lane's next rows differs by
+            const uint32_t x1 = rows == 2 ? 32 : 64, x2 = rows == 2 ? 64 : 0, x3 = rows == 2 ? 96 : 64, pace = rows * 128;
+            const float *g = which == 0 && a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr;
+            float total = 0.0f;
+            bool any = false;
+            float2 next = make_float2(0.0f, 0.0f);
+            auto decays = [&](int i) {              // of token i and the next one, 0 past the end
+                float2 f = make_float2(0.0f, 0.0f);
+                if (g && i < w.n) f.x = g[i * a.g.token];
+                if (g && i + 1 < w.n) f.y = g[(i + 1) * a.g.token];
+                return f;
+            };
             int stage = 0;
-            uint32_t phase = 0;
+            uint32_t phase = 1;                     // (the first waits for empty stages return at once)
+            next = decays(2 * lane);
 #pragma unroll 1
             for (int n = 0; n < N; n++) {
-                if (n >= stages) wait(&empty[stage], phase ^ 1);
+                wait(&empty[stage], phase);
                 const int m = min(C, w.n - n * C);
+                if (copies) {
+                    uint32_t d0 = dst + stage * STAGE;
+                    if (vec && m == C && bytes > 0) {
+                        uint32_t d1 = (d0 ^ x1) + pace, d2 = (d0 ^ x2) + 2 * pace, d3 = (d0 ^ x3) + 3 * pace;
+                        const char *from = src;
 #pragma unroll 1
-                for (int which = STATES_ONLY ? 1 : 0; which < 3; which++) {     // q, k, v
-                    const TokenView &view = which == 0 ? a.q : which == 1 ? a.k : a.v;
-                    const int width = which == 2 ? a.dv : a.dk, per = width > 64 ? 16 : 8, step = 32 * LOAD_WARPS / per;
-                    const int c = t & (per - 1), r0 = t / per, bytes = 2 * min(8, width - c * 8);
-                    if (bytes <= 0) continue;
-                    // the swizzle of row r0 + i * step: that of r0, with its upper bit inverted for the odd ones of steps of four
-                    const uint32_t dst = smem_u32(smem + stage * STAGE + (which == 2 ? 2 * KH : which == 0 ? KH : 0) * HALF_TILE + (c >> 3) * HALF_TILE) + r0 * 128;
-                    uint32_t d0 = dst + (((c & 7) ^ r0) << 4), d1 = dst + step * 128 + (((c & 7) ^ (r0 + step & 7)) << 4);
-                    const long long token = view.token * 2;
-                    const char *first = (const char *)view.p + 2 * token_base(a, view, w.b, w.s, which == 2 ? w.h : w.h / a.group) +
-                                        (w.t0 + n * C) * token + c * 16;
-                    const char *src = first + r0 * token;
-                    if (p.vec[which] && m == C) {
-#pragma unroll 1
-                        for (int i = 0; i < per; i += 8) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                cp_async16(d0, src, bytes);
-                                src += step * token;
-                                cp_async16(d1, src, bytes);
-                                src += step * token;
-                                d0 += step * 256;
-                                d1 += step * 256;
-                            }
+                        for (int r = 0; r < C; r += 4 * rows) {
+                            cp_async16(d0, from, bytes);
+                            from += step;
+                            cp_async16(d1, from, bytes);
+                            from += step;
+                            cp_async16(d2, from, bytes);
+                            from += step;
+                            cp_async16(d3, from, bytes);
+                            from += step;
+                            d0 += 4 * pace, d1 += 4 * pace, d2 += 4 * pace, d3 += 4 * pace;
                         }
-                    } else {                    // of rows past the end nothing is read, zeros arrive
+                    } else if (bytes > 0) {         // of rows past the end nothing is read, zeros arrive
+                        const char *from = src, *any_row = src - r0 * pitch;
 #pragma unroll 1
-                        for (int r = r0; r < C; r += step) {
-                            if (p.vec[which]) cp_async16(d0, r < m ? src : first, r < m ? bytes : 0);
-                            else copy_values(d0, (const __nv_bfloat16 *)(r < m ? src : first), r < m ? bytes / 2 : 0);
-                            src += step * token;
-                            const uint32_t next = d0 + step * 256;
-                            d0 = d1;
-                            d1 = next;
+                        for (int r = r0; r < C; r += rows, from += step) {
+                            const uint32_t to = d0 + (r - r0) * 128 ^ (((c ^ r) & 7 ^ (c ^ r0) & 7) << 4);
+                            if (vec) cp_async16(to, r < m ? from : any_row, r < m ? bytes : 0);
+                            else copy_values(to, (const __nv_bfloat16 *)(r < m ? from : any_row), r < m ? bytes / 2 : 0);
                         }
                     }
+                    src += C * pitch;
+                    if (vec) {
+                        cp_async_arrive(&full[stage]);
+                    } else {
+                        mbar_arrive(&full[stage]);
+                    }
                 }
-                if (all_vec) {
-                    cp_async_arrive(&full[stage]);
-                } else {
-                    asm volatile("cp.async.wait_all;" ::: "memory");
+                if (which == 0) {
+                    const float2 f = next;
+                    if (n + 1 < N) next = decays((n + 1) * C + 2 * lane);
+                    Decays &d = dec[n % SLOTS];
+                    const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
+                    const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
+                    float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
+                        if (lane >= o) up += u;
+                        if (lane + o < 32) down += v2;
+                    }
+                    const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1), both = even | odds;
+                    float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+                    if (lane == 0) before = 0.0f;
+                    if (lane == 31) behind = 0.0f;
+                    // (ex2 is good to 2^-22 of its value, the size of fp32 sums' errors)
+                    constexpr float LOG2E = 1.4426950408889634f;
+                    const float s0 = (before + g0) * LOG2E, s1 = up * LOG2E;
+                    float2 start = make_float2(p.scale * ex2(s0), p.scale * ex2(s1)), end = make_float2(ex2((behind + g1) * LOG2E), ex2(behind * LOG2E));
+                    if (both) {                 // nothing passes a reset
+                        const unsigned upto = 0xffffffffu >> (31 - lane);       // lanes up to this one
+                        if ((both & upto >> 1) || r0) start.x = 0.0f;
+                        if ((both & upto >> 1) || r0 || r1) start.y = 0.0f;
+                        if ((both & ~upto) || r1) end.x = 0.0f;
+                        if (both & ~upto) end.y = 0.0f;
+                    }
+                    *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0, s1);
+                    *(float2 *)(d.from_start + 2 * lane) = start;
+                    *(float2 *)(d.to_end + 2 * lane) = end;
+                    const float sum = __shfl_sync(0xffffffffu, up, 31);
+                    if (lane < 2) {             // a bit per token from a bit per pair
+                        unsigned bits = 0;
+                        if (both)
+#pragma unroll 1
+                            for (int i = 0; i < 16; i++) bits |= ((even >> (lane * 16 + i) & 1) | (odds >> (lane * 16 + i) & 1) << 1) << (2 * i);
+                        d.resets[lane] = bits;
+                        if (lane == 0) d.less = both ? -1.0f : expm1f(sum);
+                    }
+                    total += sum;
+                    any = any || both != 0;
                     mbar_arrive(&full[stage]);
                 }
                 if (++stage == stages) stage = 0, phase ^= 1;
             }
+            if (STATES_ONLY && which == 0 && lane == 0 && served)
+                p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
             asm volatile("cp.async.wait_all;" ::: "memory");
             tc_fence_before();
             __syncthreads();
-        } else if (warp == DECAY_WARP) {
-            // ------------------------------------------------------------ decays
-            const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) : nullptr;
-            int stage = 0;
-            uint32_t phase = 0;
-            float total = 0.0f;
-            bool any = false;
-            float2 next = make_float2(0.0f, 0.0f);
-            auto decays = [&](int n) {              // of tokens 2 * lane and the one behind it, 0 past the end
-                const int i = n * C + 2 * lane;
-                float2 f = make_float2(0.0f, 0.0f);
-                if (g && i < w.n) f.x = g[(w.t0 + i) * a.g.token];
-                if (g && i + 1 < w.n) f.y = g[(w.t0 + i + 1) * a.g.token];
-                return f;
-            };
-            if (N > 0) next = decays(0);
-            for (int n = 0; n < N; n++) {
-                if (n >= stages) wait(&empty[stage], phase ^ 1);
-                const float2 f = next;
-                if (n + 1 < N) next = decays(n + 1);
-                Decays &d = dec[n % SLOTS];
-                const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
-                const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
-                float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
-                    if (lane >= o) up += u;
-                    if (lane + o < 32) down += v2;
-                }
-                const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1);
-                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-                if (lane == 0) before = 0.0f;
-                if (lane == 31) behind = 0.0f;
-                const unsigned upto = 0xffffffffu >> (31 - lane), under = upto >> 1;        // lanes up to this one; below it
-                const bool reset_before = ((even | odds) & under) != 0, reset_behind = ((even | odds) & ~upto) != 0;
-                const float s0 = before + g0;
-                constexpr float LOG2E = 1.4426950408889634f;
-                *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0 * LOG2E, up * LOG2E);
-                *(float2 *)(d.from_start + 2 * lane) =
-                    make_float2(reset_before || r0 ? 0.0f : p.scale * expf(s0), reset_before || r0 || r1 ? 0.0f : p.scale * expf(up));
-                *(float2 *)(d.to_end + 2 * lane) = make_float2(reset_behind || r1 ? 0.0f : expf(behind + g1), reset_behind ? 0.0f : expf(behind));
-                // a bit per token from a bit per pair
-                unsigned long long bits = 0;
-                if ((even | odds) != 0 && lane == 0)
-#pragma unroll 1
-                    for (int i = 0; i < 32; i++) bits |= (unsigned long long)((even >> i & 1) | (odds >> i & 1) << 1) << (2 * i);
-                const float sum = __shfl_sync(0xffffffffu, up, 31);
-                if (lane == 0) {
-                    d.resets[0] = (unsigned)bits;
-                    d.resets[1] = (unsigned)(bits >> 32);
-                    d.less = (even | odds) ? -1.0f : expm1f(sum);
-                }
-                total += sum;
-                any = any || (even | odds) != 0;
-                mbar_arrive(&full[stage]);
-                if (++stage == stages) stage = 0, phase ^= 1;
-            }
-            if (STATES_ONLY && lane == 0 && served)
-                p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
-            tc_fence_before();
-            __syncthreads();
         } else {
-            // ------------------------------------------------------------ MMAs, by one thread
-            if (lane == 0 && N > 0) {
-                int stage = 0, next_stage = 0;
-                uint32_t next_phase = 0;
-                const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0;
-                const uint32_t negative = p.negative << 13;         // of A: a negative scale
-                auto wait1 = [&](uint64_t *bar, uint32_t parity) {
-                    if (!mbar_try_wait(bar, parity)) wait_long(smem_u32(bar), parity, abort_flag, p.status);
-                };
+            // ------------------------------------------------------------ MMAs
+            const uint32_t leader = elect_one();
+            const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0, negative = p.negative << 13;     // of A: a negative scale
+            int stage = 0, next_stage = 0;
+            uint32_t next_phase = 0;
 #pragma unroll 1
-                for (int n = -1; n < N; n++) {
-                    const uint32_t k = smem_u32(smem + stage * STAGE), q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
-                    if (n >= 0) {
-                        wait1(v_full, n & 1);
-                        tc_fence_after();
+            for (int n = -1; n < N; n++) {
+                const uint32_t k = smem_u32(smem) + stage * STAGE, q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
+                if (n >= 0) {
+                    wait(v_full, n & 1);
+                    wait(d_empty, (n - 1) & 1);         // (at first: at once, and so below)
+                    tc_fence_after();
 #pragma unroll 1
-                        for (int term = 2; term >= 0; term--)
+                    for (int term = 2; term >= 0; term--)
 #pragma unroll
-                            for (int i = 0; i < C / 16; i++)
-                                umma_bf16_ts(tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
-                                             idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
-                        umma_commit(d_full);
-                    }
-                    if (n + 1 < N) {
-                        // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
-                        wait1(&full[next_stage], next_phase);
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        if (!STATES_ONLY) {
-                            if (n >= 0) wait1(kq_empty, n & 1);
-                            tc_fence_after();
-                            const uint32_t k1 = smem_u32(smem + next_stage * STAGE);
-#pragma unroll 1
-                            for (int h = 0; h < KH; h++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    umma_bf16(tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
-                                              idesc_bf16(64, C, 0, 0), (h | i) != 0);
-                            umma_commit(kq_full);
-                        }
-                        if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
-                    }
-                    if (n < 0) continue;
+                        for (int i = 0; i < C / 16; i++)
+                            umma_bf16_ts(leader, tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
+                                         idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
+                    umma_done(leader, d_full);
+                }
+                if (n + 1 < N) {
+                    // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
+                    wait(&full[next_stage], next_phase);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     if (!STATES_ONLY) {
-                        wait1(s_full, n & 1);
-                        if (n > 0) wait1(o_empty, (n - 1) & 1);
+                        wait(kq_empty, n & 1);
                         tc_fence_after();
+                        const uint32_t k1 = smem_u32(smem) + next_stage * STAGE;
 #pragma unroll 1
                         for (int h = 0; h < KH; h++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                umma_bf16_ts(tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
-                                             idesc_bf16(128, C, 0, 0), (h | i) != 0);
-                        umma_commit(s_empty);
-                        wait1(&p_full[n & 1], n >> 1 & 1);
-                        const uint32_t pt = smem_u32(P + (n & 1) * HALF_TILE);
-#pragma unroll
-                        for (int i = 0; i < C / 16; i++)
-                            umma_bf16(tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE),
-                                      idesc_bf16(128, C, 1, 1) | negative, i != 0);
-                        umma_commit(o_full);
+                                umma_bf16(leader, tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
+                                          idesc_bf16(64, C, 0, 0), (h | i) != 0);
+                        umma_done(leader, kq_full);
                     }
-                    umma_commit(&empty[stage]);
-                    if (++stage == stages) stage = 0;
+                    if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
                 }
+                if (n < 0) continue;
+                if (!STATES_ONLY) {
+                    wait(s_full, n & 1);
+                    wait(o_empty, (n - 1) & 1);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int h = 0; h < KH; h++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            umma_bf16_ts(leader, tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
+                                         idesc_bf16(128, C, 0, 0), (h | i) != 0);
+                    umma_done(leader, s_empty);
+                    wait(&p_full[n & 1], n >> 1 & 1);
+                    const uint32_t pt = smem_u32(P) + (n & 1) * HALF_TILE;
+#pragma unroll
+                    for (int i = 0; i < C / 16; i++)
+                        umma_bf16(leader, tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE),
+                                  idesc_bf16(128, C, 1, 1) | negative, i != 0);
+                    umma_done(leader, o_full);
+                }
+                umma_done(leader, &empty[stage]);
+                if (++stage == stages) stage = 0;
             }
-            __syncwarp();
             tc_fence_before();
             __syncthreads();
         }
