@@ -33,12 +33,12 @@ using namespace tc;
 namespace {
 
 constexpr int C = 64;                       // tokens of a chunk
-// Roles by warpgroup: two for the state, two for V's weighted terms, one each for the weights of pairs and for the outputs; then a
-// warp of loads for each of Q (and the decays), K and V, and the one that issues MMAs.  Many warps of few registers: what they do is a chain of short
+// Roles by warpgroup: two for the state, two for V's weighted terms, one each for the weights of pairs and for the outputs; then two
+// warps of loads, one for the decays, and the one that issues MMAs.  Many warps of few registers: what they do is a chain of short
 // steps, and with four warps to a scheduler (state and terms in one role, weights and outputs in another) a chunk took 4300 cycles.
-constexpr int STATE_WARPS = 8, TERM_WARPS = 8, PAIR_WARPS = 4, OUT_WARPS = 4, LOAD_WARPS = 3;
+constexpr int STATE_WARPS = 8, TERM_WARPS = 8, PAIR_WARPS = 4, OUT_WARPS = 4, LOAD_WARPS = 2;
 constexpr int TERM0 = STATE_WARPS, PAIR0 = TERM0 + TERM_WARPS, OUT0 = PAIR0 + PAIR_WARPS, LOAD0 = OUT0 + OUT_WARPS;
-constexpr int MMA_WARP = LOAD0 + LOAD_WARPS;
+constexpr int DECAY_WARP = LOAD0 + LOAD_WARPS, MMA_WARP = DECAY_WARP + 1;
 constexpr int THREADS = 32 * (MMA_WARP + 1);
 // Registers of a thread: what a launch of so many threads gets, and how the warpgroups share it (their sum is at most seven times that)
 constexpr int REGS = 72, STATE_REGS = 104, TERM_REGS = 64, PAIR_REGS = 56, OUT_REGS = 56, OTHER_REGS = 56;
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     grid_dependents_start();
     if (tid == 0) {
         for (int s = 0; s < MAX_STAGES; s++) {
-            mbar_init(&full[s], 32 * (STATES_ONLY ? 2 : 3) + 32);      // a copy from each lane of the loading warps, and the decays
+            mbar_init(&full[s], 32 * LOAD_WARPS + 32);
             mbar_init(&empty[s], 1);
         }
         mbar_init(kq_full, 1);
@@ -588,120 +588,147 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         more_registers<REGS>();
     } else {
         fewer_registers<OTHER_REGS>();
-        if (warp < MMA_WARP) {
-            // ------------------------------------------------------------ loads, and the decays
-            // A warp copies a tile of one tensor (q, k, v): a lane one 16-byte group of every second row (of four, where rows are of up to
-            // eight groups).
-            const int which = warp - LOAD0;
-            const bool copies = !STATES_ONLY || which != 0;
-            const TokenView &view = which == 0 ? a.q : which == 1 ? a.k : a.v;
-            const int width = which == 2 ? a.dv : a.dk, rows = width > 64 ? 2 : 4;
-            const int c = width > 64 ? lane & 15 : lane & 7, r0 = width > 64 ? lane >> 4 : lane >> 3, bytes = 2 * min(8, width - c * 8);
-            const bool vec = p.vec[which];
-            const long long pitch = view.token * 2, step = rows * pitch;
-            const char *src = (const char *)view.p + 2 * (token_base(a, view, w.b, w.s, which == 2 ? w.h : w.h / a.group) + (w.t0 + r0) * view.token) + c * 16;
-            const uint32_t dst = smem_u32(smem) + (which == 0 ? KH : which == 1 ? 0 : 2 * KH) * HALF_TILE + (c >> 3) * HALF_TILE + r0 * 128 + (((c & 7) ^ r0) << 4);
-            // what the swizzle of the lane's next rows differs by
-            const uint32_t x1 = rows == 2 ? 32 : 64, x2 = rows == 2 ? 64 : 0, x3 = rows == 2 ? 96 : 64, pace = rows * 128;
-            const float *g = which == 0 && a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr;
+        if (warp < DECAY_WARP) {
+            // ------------------------------------------------------------ loads
+            // One warp copies K and the first half of Q, the other V and the second half of Q: a lane one 16-byte group of every second row
+            // (of four, where rows are of up to eight groups).
+            struct Copy {
+                const char *src;            // the lane's group of its first row of the next chunk
+                long long pitch;            // bytes from row to row
+                uint32_t dst;               // in stage 0
+                int bytes, rows;            // of the group, up to 16 (0 and less: none); rows of a warp's copy
+                bool vec;
+            };
+            auto copy_of = [&](const TokenView &view, int head, int width, bool vec, int tile, int from_row) {
+                Copy y;
+                y.rows = width > 64 ? 2 : 4;
+                const int c = width > 64 ? lane & 15 : lane & 7, r0 = width > 64 ? lane >> 4 : lane >> 3;
+                y.bytes = 2 * min(8, width - c * 8);
+                y.vec = vec;
+                y.pitch = view.token * 2;
+                y.src = (const char *)view.p + 2 * (token_base(a, view, w.b, w.s, head) + (w.t0 + from_row + r0) * view.token) + c * 16;
+                y.dst = smem_u32(smem) + (tile + (c >> 3)) * HALF_TILE + (from_row + r0) * 128 + (((c & 7) ^ r0) << 4);
+                return y;
+            };
+            const bool second = warp != LOAD0;
+            const Copy own = second ? copy_of(a.v, w.h, a.dv, p.vec[2], 2 * KH, 0) : copy_of(a.k, w.h / a.group, a.dk, p.vec[1], 0, 0);
+            const Copy shared = copy_of(a.q, w.h / a.group, a.dk, p.vec[0], KH, second ? C / 2 : 0);
+            const bool all_vec = own.vec && (STATES_ONLY || shared.vec);
+            long long chunk = 0;            // tokens in front of this one
+            int stage = 0;
+            uint32_t phase = 1;             // (the first waits for empty stages return at once)
+#pragma unroll 1
+            for (int n = 0; n < N; n++, chunk += C) {
+                wait(&empty[stage], phase);
+#pragma unroll 1
+                for (int i = 0; i < (STATES_ONLY ? 1 : 2); i++) {
+                    const Copy y = i == 0 ? own : shared;
+                    const int from_row = i == 1 && second ? C / 2 : 0, rows = i == 1 ? C / 2 : C, m = min(rows, w.n - (int)chunk - from_row);
+                    const char *src = y.src + chunk * y.pitch;
+                    const long long step = y.rows * y.pitch;
+                    const uint32_t pace = y.rows * 128;
+                    uint32_t d0 = y.dst + stage * STAGE;
+                    if (y.bytes <= 0) continue;
+                    if (y.vec && m == rows) {
+                        // what the swizzle of the lane's next rows differs by
+                        uint32_t d1 = (d0 ^ (y.rows == 2 ? 32 : 64)) + pace, d2 = (d0 ^ (y.rows == 2 ? 64 : 0)) + 2 * pace,
+                                 d3 = (d0 ^ (y.rows == 2 ? 96 : 64)) + 3 * pace;
+                        // four addresses, so that one's next value need not wait for the copy that is still reading it
+                        const char *s1 = src + step, *s2 = s1 + step, *s3 = s2 + step;
+#pragma unroll 1
+                        for (int r = 0; r < rows; r += 4 * y.rows) {
+                            cp_async16(d0, src, y.bytes);
+                            cp_async16(d1, s1, y.bytes);
+                            cp_async16(d2, s2, y.bytes);
+                            cp_async16(d3, s3, y.bytes);
+                            src += 4 * step, s1 += 4 * step, s2 += 4 * step, s3 += 4 * step;
+                            d0 += 4 * pace, d1 += 4 * pace, d2 += 4 * pace, d3 += 4 * pace;
+                        }
+                    } else {                // of rows past the end nothing is read, zeros arrive
+                        const int r0 = y.rows == 2 ? lane >> 4 : lane >> 3;
+                        const char *any_row = y.src + ((long long)w.n - 1 - from_row - r0) * y.pitch;      // the last token
+#pragma unroll 1
+                        for (int r = r0; r < rows; r += y.rows, src += step) {
+                            const uint32_t to = d0 + (r - r0) * 128 ^ ((r ^ r0) & 7) << 4;
+                            if (y.vec) cp_async16(to, r < m ? src : any_row, r < m ? y.bytes : 0);
+                            else copy_values(to, (const __nv_bfloat16 *)(r < m ? src : any_row), r < m ? y.bytes / 2 : 0);
+                        }
+                    }
+                }
+                if (all_vec) {
+                    cp_async_arrive(&full[stage]);
+                } else {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    mbar_arrive(&full[stage]);
+                }
+                if (++stage == stages) stage = 0, phase ^= 1;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            tc_fence_before();
+            __syncthreads();
+        } else if (warp == DECAY_WARP) {
+            // ------------------------------------------------------------ decays
+            const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr;
             float total = 0.0f;
             bool any = false;
-            float2 next = make_float2(0.0f, 0.0f);
             auto decays = [&](int i) {              // of token i and the next one, 0 past the end
                 float2 f = make_float2(0.0f, 0.0f);
                 if (g && i < w.n) f.x = g[i * a.g.token];
                 if (g && i + 1 < w.n) f.y = g[(i + 1) * a.g.token];
                 return f;
             };
+            float2 next = decays(2 * lane);
             int stage = 0;
-            uint32_t phase = 1;                     // (the first waits for empty stages return at once)
-            next = decays(2 * lane);
+            uint32_t phase = 1;
 #pragma unroll 1
             for (int n = 0; n < N; n++) {
                 wait(&empty[stage], phase);
-                const int m = min(C, w.n - n * C);
-                if (copies) {
-                    uint32_t d0 = dst + stage * STAGE;
-                    if (vec && m == C && bytes > 0) {
-                        uint32_t d1 = (d0 ^ x1) + pace, d2 = (d0 ^ x2) + 2 * pace, d3 = (d0 ^ x3) + 3 * pace;
-                        const char *from = src;
-#pragma unroll 1
-                        for (int r = 0; r < C; r += 4 * rows) {
-                            cp_async16(d0, from, bytes);
-                            from += step;
-                            cp_async16(d1, from, bytes);
-                            from += step;
-                            cp_async16(d2, from, bytes);
-                            from += step;
-                            cp_async16(d3, from, bytes);
-                            from += step;
-                            d0 += 4 * pace, d1 += 4 * pace, d2 += 4 * pace, d3 += 4 * pace;
-                        }
-                    } else if (bytes > 0) {         // of rows past the end nothing is read, zeros arrive
-                        const char *from = src, *any_row = src - r0 * pitch;
-#pragma unroll 1
-                        for (int r = r0; r < C; r += rows, from += step) {
-                            const uint32_t to = d0 + (r - r0) * 128 ^ (((c ^ r) & 7 ^ (c ^ r0) & 7) << 4);
-                            if (vec) cp_async16(to, r < m ? from : any_row, r < m ? bytes : 0);
-                            else copy_values(to, (const __nv_bfloat16 *)(r < m ? from : any_row), r < m ? bytes / 2 : 0);
-                        }
-                    }
-                    src += C * pitch;
-                    if (vec) {
-                        cp_async_arrive(&full[stage]);
-                    } else {
-                        mbar_arrive(&full[stage]);
-                    }
-                }
-                if (which == 0) {
-                    const float2 f = next;
-                    if (n + 1 < N) next = decays((n + 1) * C + 2 * lane);
-                    Decays &d = dec[n % SLOTS];
-                    const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
-                    const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
-                    float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
+                const float2 f = next;
+                if (n + 1 < N) next = decays((n + 1) * C + 2 * lane);
+                Decays &d = dec[n % SLOTS];
+                const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
+                const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
+                float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
-                        if (lane >= o) up += u;
-                        if (lane + o < 32) down += v2;
-                    }
-                    const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1), both = even | odds;
-                    float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-                    if (lane == 0) before = 0.0f;
-                    if (lane == 31) behind = 0.0f;
-                    // (ex2 is good to 2^-22 of its value, the size of fp32 sums' errors)
-                    constexpr float LOG2E = 1.4426950408889634f;
-                    const float s0 = (before + g0) * LOG2E, s1 = up * LOG2E;
-                    float2 start = make_float2(p.scale * ex2(s0), p.scale * ex2(s1)), end = make_float2(ex2((behind + g1) * LOG2E), ex2(behind * LOG2E));
-                    if (both) {                 // nothing passes a reset
-                        const unsigned upto = 0xffffffffu >> (31 - lane);       // lanes up to this one
-                        if ((both & upto >> 1) || r0) start.x = 0.0f;
-                        if ((both & upto >> 1) || r0 || r1) start.y = 0.0f;
-                        if ((both & ~upto) || r1) end.x = 0.0f;
-                        if (both & ~upto) end.y = 0.0f;
-                    }
-                    *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0, s1);
-                    *(float2 *)(d.from_start + 2 * lane) = start;
-                    *(float2 *)(d.to_end + 2 * lane) = end;
-                    const float sum = __shfl_sync(0xffffffffu, up, 31);
-                    if (lane < 2) {             // a bit per token from a bit per pair
-                        unsigned bits = 0;
-                        if (both)
-#pragma unroll 1
-                            for (int i = 0; i < 16; i++) bits |= ((even >> (lane * 16 + i) & 1) | (odds >> (lane * 16 + i) & 1) << 1) << (2 * i);
-                        d.resets[lane] = bits;
-                        if (lane == 0) d.less = both ? -1.0f : expm1f(sum);
-                    }
-                    total += sum;
-                    any = any || both != 0;
-                    mbar_arrive(&full[stage]);
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
+                    if (lane >= o) up += u;
+                    if (lane + o < 32) down += v2;
                 }
+                const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1), both = even | odds;
+                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+                if (lane == 0) before = 0.0f;
+                if (lane == 31) behind = 0.0f;
+                // (ex2 is good to 2^-22 of its value, the size of fp32 sums' errors)
+                constexpr float LOG2E = 1.4426950408889634f;
+                const float s0 = (before + g0) * LOG2E, s1 = up * LOG2E;
+                float2 start = make_float2(p.scale * ex2(s0), p.scale * ex2(s1)), end = make_float2(ex2((behind + g1) * LOG2E), ex2(behind * LOG2E));
+                if (both) {                 // nothing passes a reset
+                    const unsigned upto = 0xffffffffu >> (31 - lane);       // lanes up to this one
+                    if ((both & upto >> 1) || r0) start.x = 0.0f;
+                    if ((both & upto >> 1) || r0 || r1) start.y = 0.0f;
+                    if ((both & ~upto) || r1) end.x = 0.0f;
+                    if (both & ~upto) end.y = 0.0f;
+                }
+                *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0, s1);
+                *(float2 *)(d.from_start + 2 * lane) = start;
+                *(float2 *)(d.to_end + 2 * lane) = end;
+                const float sum = __shfl_sync(0xffffffffu, up, 31);
+                if (lane < 2) {             // a bit per token from a bit per pair
+                    unsigned bits = 0;
+                    if (both)
+#pragma unroll 1
+                        for (int i = 0; i < 16; i++) bits |= ((even >> (lane * 16 + i) & 1) | (odds >> (lane * 16 + i) & 1) << 1) << (2 * i);
+                    d.resets[lane] = bits;
+                    if (lane == 0) d.less = both ? -1.0f : expm1f(sum);
+                }
+                total += sum;
+                any = any || both != 0;
+                mbar_arrive(&full[stage]);
                 if (++stage == stages) stage = 0, phase ^= 1;
             }
-            if (STATES_ONLY && which == 0 && lane == 0 && served)
+            if (STATES_ONLY && lane == 0 && served)
                 p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
-            asm volatile("cp.async.wait_all;" ::: "memory");
             tc_fence_before();
             __syncthreads();
         } else {
