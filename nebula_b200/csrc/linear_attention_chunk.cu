@@ -113,24 +113,36 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t mn_step) {
     return ((uint64_t)SMEM_DESC_HI << 32) | ((addr >> 4) & 0x3FFF) | ((mn_step >> 4) << 16);
 }
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t *v) {
-    __syncwarp();
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]),
         "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
         "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
         : "memory");
 }
+// (The roles' warps run converged: every wait ends with that.)
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 16 lanes of tensor memory in the layout of matrix fragments: thread t holds rows t / 4 and t / 4 + 8.  Loads: of every eight columns
 // 2 (t % 4) and the next one, of both rows; stores of four columns: column t % 4, of both rows.
 __device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t (&v)[8]) {
-    __syncwarp();
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                  : "r"(taddr)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t (&v)[16]) {
-    __syncwarp();
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
@@ -139,7 +151,6 @@ __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t (&v)[
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t *v) {
-    __syncwarp();
     asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr)
                  : "memory");
@@ -194,7 +205,7 @@ struct Waits {
     volatile int *abort_flag;
     int *status;
     __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const {
-        if (!mbar_try_wait(bar, parity)) wait_long(smem_u32(bar), parity, abort_flag, status);
+        if (!mbar_try_wait_parked(bar, parity, 20000u)) wait_long(smem_u32(bar), parity, abort_flag, status);
         __syncwarp();
     }
 };
@@ -376,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     for (int i = 0; i < 16; i++) x[i] = pack_bf16(S[c + i].x, S[c + i].y);
                     tmem_st_32x16(at + T_S + half * (R / 2) + c, x);
                 }
-                tmem_st_wait();
+                tmem_stores_done();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_full);
@@ -385,14 +396,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             tc_fence_after();
             const float less = dec[n % SLOTS].less;
 #pragma unroll
-            for (int c = 0; c < R; c += 16) {
-                uint32_t d[16];
-                tmem_ld_32x16(at + T_D + half * R + c, d);
-                tmem_ld_wait();
+            for (int c = 0; c < R; c += 32) {
+                uint32_t d[32];
+                tmem_load_32(at + T_D + half * R + c, d);
+                tmem_loads_done();
                 // as S + (less S + new): what a decay near 1 takes away keeps its own precision.  Once a value is not finite it
                 // stays so, whatever the decays
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < 16; i++) {
                     float2 &x = S[c / 2 + i];
                     x = add2(x, fma2(make_float2(less, less), x, as_float2(d[2 * i], d[2 * i + 1])));
                 }
@@ -456,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                         tmem_st_16x128_x4(at + ((uint32_t)(h * 16) << 16) + term * 32, y);
                     }
                 }
-                tmem_st_wait();
+                tmem_stores_done();
             } else {
                 wait(d_full, (n - 1) & 1);
             }
@@ -495,7 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     tmem_ld_16x256_x2(at + g * 8, x);
                     const float2 s = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + i1), t = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + 8 + i1);
                     const float e[8] = {ex2(s.x + m0), ex2(s.y + m0), ex2(s.x + m1), ex2(s.y + m1), ex2(t.x + m0), ex2(t.y + m0), ex2(t.x + m1), ex2(t.y + m1)};
-                    tmem_ld_wait();
+                    tmem_loads_done();
                     uint32_t y[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) y[i] = pack_bf16(__uint_as_float(x[2 * i]) * e[2 * i], __uint_as_float(x[2 * i + 1]) * e[2 * i + 1]);
@@ -547,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                         uint32_t x[16], y[16];
                         tmem_ld_16x256_x4(from + T_O2, x);
                         tmem_ld_16x256_x4(from + T_O1, y);
-                        tmem_ld_wait();
+                        tmem_loads_done();
 #pragma unroll
                         for (int g = 0; g < 4; g++) {
                             const float2 e = *(const float2 *)(weight + (h & 1) * 32 + g * 8);
