@@ -34,11 +34,12 @@ namespace {
 
 constexpr int C = 64;                       // tokens of a chunk
 // Roles by warpgroup: two for the state, two for V's weighted terms, one each for the weights of pairs and for the outputs; then two
-// warps of loads, one for the decays, and the one that issues MMAs.  Many warps of few registers: what they do is a chain of short
+// warps of loads, and two that issue MMAs (those of the state, and the others).  Many warps of few registers: what they do is a chain of short
 // steps, and with four warps to a scheduler (state and terms in one role, weights and outputs in another) a chunk took 4300 cycles.
 constexpr int STATE_WARPS = 8, TERM_WARPS = 8, PAIR_WARPS = 4, OUT_WARPS = 4, LOAD_WARPS = 2;
 constexpr int TERM0 = STATE_WARPS, PAIR0 = TERM0 + TERM_WARPS, OUT0 = PAIR0 + PAIR_WARPS, LOAD0 = OUT0 + OUT_WARPS;
-constexpr int DECAY_WARP = LOAD0 + LOAD_WARPS, MMA_WARP = DECAY_WARP + 1;
+constexpr int DECAY_WARP = OUT0 - 1;        // one of the pairs' warps
+constexpr int STATE_MMA_WARP = LOAD0 + LOAD_WARPS, MMA_WARP = STATE_MMA_WARP + 1;
 constexpr int THREADS = 32 * (MMA_WARP + 1);
 // Registers of a thread: what a launch of so many threads gets, and how the warpgroups share it (their sum is at most seven times that)
 constexpr int REGS = 72, STATE_REGS = 104, TERM_REGS = 64, PAIR_REGS = 56, OUT_REGS = 56, OTHER_REGS = 56;
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     if (tid == 0) {
         for (int s = 0; s < MAX_STAGES; s++) {
             mbar_init(&full[s], 32 * LOAD_WARPS + 32);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], STATES_ONLY ? 1 : 2);      // both warps that issue MMAs
         }
         mbar_init(kq_full, 1);
         mbar_init(kq_empty, PAIR_WARPS);
@@ -482,6 +483,73 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     } else if (warp < OUT0) {
         // ------------------------------------------------------------ weights of pairs
         fewer_registers<PAIR_REGS>();
+        // ------------------------------------------------------------ decays: the last warp, which has the fewest pairs
+        const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr;
+        auto load_decays = [&](int i) {             // of token i and the next one, 0 past the end
+            float2 f = make_float2(0.0f, 0.0f);
+            if (g && i < w.n) f.x = g[i * a.g.token];
+            if (g && i + 1 < w.n) f.y = g[(i + 1) * a.g.token];
+            return f;
+        };
+        float2 next = warp == DECAY_WARP && N > 0 ? load_decays(2 * lane) : make_float2(0.0f, 0.0f);
+        float total = 0.0f;
+        bool any = false;
+        auto decays = [&](int n) {
+            const float2 f = next;
+            if (n + 1 < N) next = load_decays((n + 1) * C + 2 * lane);
+            Decays &d = dec[n % SLOTS];
+            const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
+            const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
+            float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
+                if (lane >= o) up += u;
+                if (lane + o < 32) down += v2;
+            }
+            const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1), both = even | odds;
+            float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+            if (lane == 0) before = 0.0f;
+            if (lane == 31) behind = 0.0f;
+            // (ex2 is good to 2^-22 of its value, the size of fp32 sums' errors)
+            constexpr float LOG2E = 1.4426950408889634f;
+            const float s0 = (before + g0) * LOG2E, s1 = up * LOG2E;
+            float2 start = make_float2(p.scale * ex2(s0), p.scale * ex2(s1)), end = make_float2(ex2((behind + g1) * LOG2E), ex2(behind * LOG2E));
+            if (both) {                 // nothing passes a reset
+                const unsigned upto = 0xffffffffu >> (31 - lane);       // lanes up to this one
+                if ((both & upto >> 1) || r0) start.x = 0.0f;
+                if ((both & upto >> 1) || r0 || r1) start.y = 0.0f;
+                if ((both & ~upto) || r1) end.x = 0.0f;
+                if (both & ~upto) end.y = 0.0f;
+            }
+            *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0, s1);
+            *(float2 *)(d.from_start + 2 * lane) = start;
+            *(float2 *)(d.to_end + 2 * lane) = end;
+            const float sum = __shfl_sync(0xffffffffu, up, 31);
+            if (lane < 2) {             // a bit per token from a bit per pair
+                unsigned bits = 0;
+                if (both)
+#pragma unroll 1
+                    for (int i = 0; i < 16; i++) bits |= ((even >> (lane * 16 + i) & 1) | (odds >> (lane * 16 + i) & 1) << 1) << (2 * i);
+                d.resets[lane] = bits;
+                if (lane == 0) d.less = both ? -1.0f : expm1f(sum);
+            }
+            total += sum;
+            any = any || both != 0;
+            mbar_arrive(&full[n % stages]);
+        };
+        if (STATES_ONLY && warp == DECAY_WARP) {
+            int stage = 0;
+            uint32_t phase = 1;
+#pragma unroll 1
+            for (int n = 0; n < N; n++) {
+                wait(&empty[stage], phase);
+                if (++stage == stages) stage = 0, phase ^= 1;
+                decays(n);
+            }
+            if (lane == 0 && served)
+                p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
+        }
         if (!STATES_ONLY) {
             const int quarter = warp & 3;
             const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + T_KQ + quarter * 16;
@@ -491,7 +559,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             const int r = lane >> 2, i1 = 2 * (lane & 3);
             const uint32_t causal = (i1 >= r ? 0xffffu : 0u) | (i1 + 1 >= r ? 0xffff0000u : 0u);       // of eight of both on the diagonal
 #pragma unroll 1
-            for (int n = 0; n < N; n++) {
+            for (int n = -2; n < N; n++) {
+                // two chunks ahead: what was in that slot, six chunks ago, and in that phase of the barrier, is done with
+                if (warp == DECAY_WARP && n + 2 < N) decays(n + 2);
+                if (n < 0) continue;
                 wait(&full[stage], phase);
                 if (++stage == stages) stage = 0, phase ^= 1;
                 const Decays &d = dec[n % SLOTS];
@@ -599,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         more_registers<REGS>();
     } else {
         fewer_registers<OTHER_REGS>();
-        if (warp < DECAY_WARP) {
+        if (warp < STATE_MMA_WARP) {
             // ------------------------------------------------------------ loads
             // One warp copies K and the first half of Q, the other V and the second half of Q: a lane one 16-byte group of every second row
             // (of four, where rows are of up to eight groups).
@@ -677,121 +748,60 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             asm volatile("cp.async.wait_all;" ::: "memory");
             tc_fence_before();
             __syncthreads();
-        } else if (warp == DECAY_WARP) {
-            // ------------------------------------------------------------ decays
-            const float *g = a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr;
-            float total = 0.0f;
-            bool any = false;
-            auto decays = [&](int i) {              // of token i and the next one, 0 past the end
-                float2 f = make_float2(0.0f, 0.0f);
-                if (g && i < w.n) f.x = g[i * a.g.token];
-                if (g && i + 1 < w.n) f.y = g[(i + 1) * a.g.token];
-                return f;
-            };
-            float2 next = decays(2 * lane);
-            int stage = 0;
-            uint32_t phase = 1;
-#pragma unroll 1
-            for (int n = 0; n < N; n++) {
-                wait(&empty[stage], phase);
-                const float2 f = next;
-                if (n + 1 < N) next = decays((n + 1) * C + 2 * lane);
-                Decays &d = dec[n % SLOTS];
-                const bool r0 = f.x <= RESET, r1 = f.y <= RESET;
-                const float g0 = r0 ? 0.0f : f.x, g1 = r1 ? 0.0f : f.y;
-                float up = g0 + g1, down = up;          // inclusive sums from the start and from the end
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const float u = __shfl_up_sync(0xffffffffu, up, o), v2 = __shfl_down_sync(0xffffffffu, down, o);
-                    if (lane >= o) up += u;
-                    if (lane + o < 32) down += v2;
-                }
-                const unsigned even = __ballot_sync(0xffffffffu, r0), odds = __ballot_sync(0xffffffffu, r1), both = even | odds;
-                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-                if (lane == 0) before = 0.0f;
-                if (lane == 31) behind = 0.0f;
-                // (ex2 is good to 2^-22 of its value, the size of fp32 sums' errors)
-                constexpr float LOG2E = 1.4426950408889634f;
-                const float s0 = (before + g0) * LOG2E, s1 = up * LOG2E;
-                float2 start = make_float2(p.scale * ex2(s0), p.scale * ex2(s1)), end = make_float2(ex2((behind + g1) * LOG2E), ex2(behind * LOG2E));
-                if (both) {                 // nothing passes a reset
-                    const unsigned upto = 0xffffffffu >> (31 - lane);       // lanes up to this one
-                    if ((both & upto >> 1) || r0) start.x = 0.0f;
-                    if ((both & upto >> 1) || r0 || r1) start.y = 0.0f;
-                    if ((both & ~upto) || r1) end.x = 0.0f;
-                    if (both & ~upto) end.y = 0.0f;
-                }
-                *(float2 *)(d.sum2 + 2 * lane) = make_float2(s0, s1);
-                *(float2 *)(d.from_start + 2 * lane) = start;
-                *(float2 *)(d.to_end + 2 * lane) = end;
-                const float sum = __shfl_sync(0xffffffffu, up, 31);
-                if (lane < 2) {             // a bit per token from a bit per pair
-                    unsigned bits = 0;
-                    if (both)
-#pragma unroll 1
-                        for (int i = 0; i < 16; i++) bits |= ((even >> (lane * 16 + i) & 1) | (odds >> (lane * 16 + i) & 1) << 1) << (2 * i);
-                    d.resets[lane] = bits;
-                    if (lane == 0) d.less = both ? -1.0f : expm1f(sum);
-                }
-                total += sum;
-                any = any || both != 0;
-                mbar_arrive(&full[stage]);
-                if (++stage == stages) stage = 0, phase ^= 1;
-            }
-            if (STATES_ONLY && lane == 0 && served)
-                p.ws_less[(long long)(w.b * a.H + w.h) * (p.splits - 1) + w.split] = any ? -1.0f : expm1f(total);
-            tc_fence_before();
-            __syncthreads();
         } else {
             // ------------------------------------------------------------ MMAs
             const uint32_t leader = elect_one();
             const uint32_t v_step = a.dv > 64 ? HALF_TILE : 0, negative = p.negative << 13;     // of A: a negative scale
             int stage = 0, next_stage = 0;
             uint32_t next_phase = 0;
+            // a chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
+            auto tiles = [&]() {
+                wait(&full[next_stage], next_phase);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
+            };
+            // (waits for what is released behind a chunk return at once for the first)
+            if (warp == STATE_MMA_WARP) {
 #pragma unroll 1
-            for (int n = -1; n < N; n++) {
-                const uint32_t k = smem_u32(smem) + stage * STAGE, q = k + KH * HALF_TILE, v = q + KH * HALF_TILE;
-                if (n >= 0) {
+                for (int n = 0; n < N; n++) {
+                    const uint32_t k = smem_u32(smem) + stage * STAGE;
+                    tiles();
+                    wait(d_empty, (n - 1) & 1);
                     wait(v_full, n & 1);
-                    wait(d_empty, (n - 1) & 1);         // (at first: at once, and so below)
                     tc_fence_after();
-#pragma unroll 1
+#pragma unroll
                     for (int term = 2; term >= 0; term--)
 #pragma unroll
                         for (int i = 0; i < C / 16; i++)
                             umma_bf16_ts(leader, tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
                                          idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
                     umma_done(leader, d_full);
+                    umma_done(leader, &empty[stage]);
+                    if (++stage == stages) stage = 0;
                 }
-                if (n + 1 < N) {
-                    // the next chunk's tiles are there (written by copies and stores of other threads, read by MMAs)
-                    wait(&full[next_stage], next_phase);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    if (!STATES_ONLY) {
+            } else if (!STATES_ONLY) {
+#pragma unroll 1
+                for (int n = -1; n < N; n++) {
+                    if (n + 1 < N) {
+                        const uint32_t k1 = smem_u32(smem) + next_stage * STAGE;
+                        tiles();
                         wait(kq_empty, n & 1);
                         tc_fence_after();
-                        const uint32_t k1 = smem_u32(smem) + next_stage * STAGE;
-#pragma unroll 1
-                        for (int h = 0; h < KH; h++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                umma_bf16(leader, tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
-                                          idesc_bf16(64, C, 0, 0), (h | i) != 0);
+                        for (int i = 0; i < DK / 16; i++)
+                            umma_bf16(leader, tmem + T_KQ, tile_desc(k1 + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
+                                      tile_desc(k1 + (KH + (i >> 2)) * HALF_TILE + (i & 3) * 32, 16), idesc_bf16(64, C, 0, 0), i != 0);
                         umma_done(leader, kq_full);
                     }
-                    if (++next_stage == stages) next_stage = 0, next_phase ^= 1;
-                }
-                if (n < 0) continue;
-                if (!STATES_ONLY) {
+                    if (n < 0) continue;
+                    const uint32_t q = smem_u32(smem) + stage * STAGE + KH * HALF_TILE, v = q + KH * HALF_TILE;
                     wait(s_full, n & 1);
                     wait(o_empty, (n - 1) & 1);
                     tc_fence_after();
-#pragma unroll 1
-                    for (int h = 0; h < KH; h++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            umma_bf16_ts(leader, tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
-                                         idesc_bf16(128, C, 0, 0), (h | i) != 0);
+                    for (int i = 0; i < DK / 16; i++)
+                        umma_bf16_ts(leader, tmem + T_O2, tmem + T_S + i * 8, tile_desc(q + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
+                                     idesc_bf16(128, C, 0, 0), i != 0);
                     umma_done(leader, s_empty);
                     wait(&p_full[n & 1], n >> 1 & 1);
                     const uint32_t pt = smem_u32(P) + (n & 1) * HALF_TILE;
@@ -800,9 +810,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                         umma_bf16(leader, tmem + T_O1, tile_desc(v + i * 2048, v_step), tile_desc(pt + i * 2048, HALF_TILE),
                                   idesc_bf16(128, C, 1, 1) | negative, i != 0);
                     umma_done(leader, o_full);
+                    umma_done(leader, &empty[stage]);
+                    if (++stage == stages) stage = 0;
                 }
-                umma_done(leader, &empty[stage]);
-                if (++stage == stages) stage = 0;
             }
             tc_fence_before();
             __syncthreads();
