@@ -41,6 +41,13 @@ void check_launch(const char *what) {
     if (e != cudaSuccess) throw Error(NB_ERR_CUDA, std::string(what) + " launch: " + cudaGetErrorString(e));
 }
 
+bool extent_inside(nb_handle_s *h, const void *p, long long bytes) {
+    CUdeviceptr base = 0;
+    size_t size = 0;
+    if (!h->get_address_range || h->get_address_range(&base, &size, (CUdeviceptr)p) != CUDA_SUCCESS) return false;
+    return (uintptr_t)p + bytes <= (uintptr_t)base + size;
+}
+
 void check_extent(nb_handle_s *h, const void *p, long long lo_bytes, long long hi_bytes, const char *what) {
     if (!h->get_address_range || !p || hi_bytes <= lo_bytes) return;
     const uintptr_t q = (uintptr_t)p, a = q + lo_bytes, b = q + hi_bytes;

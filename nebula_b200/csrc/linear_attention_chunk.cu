@@ -62,7 +62,9 @@ struct Decays {
 };
 
 struct ChunkParams {
+    CUtensorMap maps[3];                // q, k, v: {values, heads, tokens, sequences}, boxes of 64 values x 64 tokens; where tma
     LinAttnParams a;
+    int tma;                            // whole chunks come by TMA
     int splits, chunks_per_split;       // of the axis of tokens
     float *ws;                          // [B*H][splits - 1][dk][dv]: states at the splits
     float *ws_less;                     // [B*H][splits - 1]: expm1 of each split's log decay
@@ -696,12 +698,35 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             const Copy own = second ? copy_of(a.v, w.h, a.dv, p.vec[2], 2 * KH, 0) : copy_of(a.k, w.h / a.group, a.dk, p.vec[1], 0, 0);
             const Copy shared = copy_of(a.q, w.h / a.group, a.dk, p.vec[0], KH, second ? C / 2 : 0);
             const bool all_vec = own.vec && (STATES_ONLY || shared.vec);
+            const int first_token = a.offsets ? (int)w.s.first + w.t0 : w.t0, sequence = a.offsets ? 0 : w.b;
             long long chunk = 0;            // tokens in front of this one
             int stage = 0;
             uint32_t phase = 1;             // (the first waits for empty stages return at once)
 #pragma unroll 1
             for (int n = 0; n < N; n++, chunk += C) {
                 wait(&empty[stage], phase);
+                if (p.tma && w.n - (int)chunk >= C) {
+                    if (lane == 0) {
+                        const uint32_t bar = smem_u32(&full[stage]), to = smem_u32(smem) + stage * STAGE;
+                        const int token = first_token + (int)chunk;
+                        if (second) {
+                            const int halves = a.dv > 64 ? 2 : 1;
+                            mbar_expect_tx(bar, halves * HALF_TILE);
+                            for (int i = 0; i < halves; i++) tma_load_4d(to + (2 * KH + i) * HALF_TILE, &p.maps[2], bar, i * 64, w.h, token, sequence);
+                        } else {
+                            mbar_expect_tx(bar, (STATES_ONLY ? 1 : 2) * KH * HALF_TILE);
+#pragma unroll
+                            for (int i = 0; i < KH; i++) tma_load_4d(to + i * HALF_TILE, &p.maps[1], bar, i * 64, w.h / a.group, token, sequence);
+                            if (!STATES_ONLY)
+#pragma unroll
+                                for (int i = 0; i < KH; i++) tma_load_4d(to + (KH + i) * HALF_TILE, &p.maps[0], bar, i * 64, w.h / a.group, token, sequence);
+                        }
+                    } else {
+                        mbar_arrive(&full[stage]);
+                    }
+                    if (++stage == stages) stage = 0, phase ^= 1;
+                    continue;
+                }
 #pragma unroll 1
                 for (int i = 0; i < (STATES_ONLY ? 1 : 2); i++) {
                     const Copy y = i == 0 ? own : shared;
@@ -879,6 +904,24 @@ void launch_chunks(nb_handle_s *h, const ChunkParams &p) {
     count_launch(h);
 }
 
+// The tensor map of a tensor of tokens.  False where it cannot have one: strides that repeat values, or the columns that its boxes
+// have past a row's last value (which arrive as zeros, but are read) not surely inside the tensor's allocation.
+bool map_tokens(nb_handle_s *h, const LinAttnParams &a, const TokenView &t, int heads, int dim, CUtensorMap *map) {
+    const long long tokens = a.offsets ? a.tokens : a.T, sequences = a.offsets ? 1 : a.B;
+    if (tokens < C) return false;
+    if ((heads > 1 && t.head == 0) || t.token == 0 || (sequences > 1 && t.batch == 0)) return false;
+    const int box = (dim + 63) / 64 * 64;
+    const long long last = (sequences - 1) * t.batch + (tokens - 1) * t.token + (heads - 1) * t.head;
+    if (box != dim && !extent_inside(h, t.p, (last + box) * 2)) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)sequences};
+    const cuuint64_t strides[3] = {(cuuint64_t)(heads > 1 ? t.head * 2 : 16), (cuuint64_t)t.token * 2, (cuuint64_t)(sequences > 1 ? t.batch * 2 : 16)};
+    for (cuuint64_t s : strides)
+        if (s >= 1ULL << 40) return false;
+    const cuuint32_t boxes[4] = {64, 1, C, 1}, steps[4] = {1, 1, 1, 1};
+    return h->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(t.p), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 bool linear_attention_chunks_supported(const nb_linear_attention_desc_t &d) {
@@ -929,6 +972,8 @@ void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAt
     p.vec[1] = whole(a.k, a.dk, true);
     p.vec[2] = whole(a.v, a.dv, true);
     p.out_vec = whole(a.out, a.dv, false);
+    p.tma = p.vec[0] && p.vec[1] && p.vec[2] && map_tokens(h, a, a.q, a.H / a.group, a.dk, &p.maps[0]) &&
+            map_tokens(h, a, a.k, a.H / a.group, a.dk, &p.maps[1]) && map_tokens(h, a, a.v, a.H, a.dv, &p.maps[2]);
     const bool wide = a.dk > 64;
     p.stages = wide ? stages_of<128>() : stages_of<64>();
     if (p.splits > 1) {

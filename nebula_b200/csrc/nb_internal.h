@@ -357,6 +357,8 @@ std::string trace_report(nb_handle_s *h);
 // Fails with NB_ERR_INVALID_ARG when [p + lo_bytes, p + hi_bytes) is not inside ONE device allocation (as the driver
 // reports it for p).  Pointers the driver does not know as an allocation (module globals, host memory) pass.
 void check_extent(nb_handle_s *h, const void *p, long long lo_bytes, long long hi_bytes, const char *what);
+// Are the `bytes` from p on surely inside one device allocation?
+bool extent_inside(nb_handle_s *h, const void *p, long long bytes);
 
 // ahead: launches `kernel` so that it may become resident while the kernel before it on the stream still runs (programmatic
 // dependent launch): the kernel executes grid_dependency_wait() before it touches memory that an earlier kernel may
