@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     wait(d_empty, (n - 1) & 1);
                     wait(v_full, n & 1);
                     tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                     for (int term = 2; term >= 0; term--)
 #pragma unroll
                         for (int i = 0; i < C / 16; i++)
@@ -812,10 +812,12 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                         tiles();
                         wait(kq_empty, n & 1);
                         tc_fence_after();
+#pragma unroll 1
+                        for (int h = 0; h < KH; h++)
 #pragma unroll
-                        for (int i = 0; i < DK / 16; i++)
-                            umma_bf16(leader, tmem + T_KQ, tile_desc(k1 + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
-                                      tile_desc(k1 + (KH + (i >> 2)) * HALF_TILE + (i & 3) * 32, 16), idesc_bf16(64, C, 0, 0), i != 0);
+                            for (int i = 0; i < 4; i++)
+                                umma_bf16(leader, tmem + T_KQ, tile_desc(k1 + h * HALF_TILE + i * 32, 16), tile_desc(k1 + (KH + h) * HALF_TILE + i * 32, 16),
+                                          idesc_bf16(64, C, 0, 0), (h | i) != 0);
                         umma_done(leader, kq_full);
                     }
                     if (n < 0) continue;
@@ -823,10 +825,12 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     wait(s_full, n & 1);
                     wait(o_empty, (n - 1) & 1);
                     tc_fence_after();
+#pragma unroll 1
+                    for (int h = 0; h < KH; h++)
 #pragma unroll
-                    for (int i = 0; i < DK / 16; i++)
-                        umma_bf16_ts(leader, tmem + T_O2, tmem + T_S + i * 8, tile_desc(q + (i >> 2) * HALF_TILE + (i & 3) * 32, 16),
-                                     idesc_bf16(128, C, 0, 0), i != 0);
+                        for (int i = 0; i < 4; i++)
+                            umma_bf16_ts(leader, tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
+                                         idesc_bf16(128, C, 0, 0), (h | i) != 0);
                     umma_done(leader, s_empty);
                     wait(&p_full[n & 1], n >> 1 & 1);
                     const uint32_t pt = smem_u32(P) + (n & 1) * HALF_TILE;
