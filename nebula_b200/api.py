@@ -202,6 +202,43 @@ def _mem(t):
     return MEM_DEVICE if t.is_cuda else MEM_HOST
 
 
+# Checks of the calls that a server makes for every token, where the binding's own time counts.
+_torch = None
+
+
+def _kind(dtype):
+    """nb_dtype of a torch dtype, -1 for another one."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return 0 if dtype is _torch.float32 else 1 if dtype is _torch.bfloat16 else -1
+
+
+def _empty_like(t):
+    return _torch.empty_like(t, memory_format=_torch.contiguous_format)
+
+
+def _rows(t, shape, dtype, width):
+    """Address and row stride of a tensor of evenly spaced rows."""
+    if t.shape != shape or t.dtype is not dtype or not t.is_cuda:
+        raise NebulaError(1, f"norm: a tensor is {tuple(t.shape)} {t.dtype}, expected {tuple(shape)} {dtype} on the device (gate and y are of "
+                             "the type of x, the sum of the residual's)")
+    if t.is_contiguous():
+        return t.data_ptr(), width
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1):
+        return t.data_ptr(), t.stride(0)
+    raise NebulaError(1, "norm: rows are contiguous, and evenly spaced in two dimensions")
+
+
+def _weights(t, width):
+    if t is None:
+        return 0
+    if t.dtype is not _torch.float32 or t.numel() != width or not t.is_contiguous() or not t.is_cuda:
+        raise NebulaError(1, "norm: weights are contiguous float32 tensors of the row's width on the device")
+    return t.data_ptr()
+
+
 class Handle:
     """One per host thread and GPU (the reference's network_t holds the
     equivalent device state, models/networks/network.cc:44-51)."""
@@ -214,6 +251,7 @@ class Handle:
         if rc != 0:
             raise NebulaError(rc, (self.lib.nb_last_error(None) or b"").decode())
         self.h = h
+        self._norm_desc, self._norm_io = (C.c_char * _NORM_DESC.size)(), (C.c_char * _NORM_IO.size)()
         self.set_math(math)
 
     def check(self, rc):
@@ -314,47 +352,29 @@ class Handle:
                            scale=1.0, channel_scale=None, next_norm="none", next_weight=None, next_bias=None, out=None, y=None):
         """s = residual + scale * channel_scale * (norm(x) * gate function(gate)) and y = next_norm(s), row by row
         (nb_norm_gate_residual); x [..., width], float32 or bfloat16, rows evenly spaced.  Returns (s, y), y None without a second
-        norm.  `out` may be the residual itself."""
-        import torch
-        width = x.shape[-1]
-        kinds = {torch.float32: 0, torch.bfloat16: 1}
-        kind = kinds.get(x.dtype)
-        if kind is None or not x.is_cuda:
+        norm.  `out` may be the residual itself, and `y` x itself."""
+        shape, dtype = x.shape, x.dtype
+        kind = _kind(dtype)
+        if kind < 0 or not x.is_cuda:
             raise NebulaError(1, "norm: x is a float32 or bfloat16 tensor on the device")
+        width = shape[-1]
+        like = x if residual is None else residual
         if out is None:
-            out = torch.empty(x.shape, device=x.device, dtype=x.dtype if residual is None else residual.dtype)
+            out = _empty_like(like)
         if y is None and next_norm != "none":
-            y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        rows = x.numel() // width if width else 0
-        a = [0] * 5
-        s = [0] * 5
-        for i, t in enumerate((x, gate, residual, out, y)):
-            if t is None:
-                continue
-            if t.shape != x.shape or t.device != x.device:
-                raise NebulaError(1, "norm: tensors of different shapes or devices")
-            if i in (1, 4) and t.dtype != x.dtype or i == 3 and residual is not None and t.dtype != residual.dtype:
-                raise NebulaError(1, "norm: gate and y have the type of x, the sum that of the residual")
-            if t.is_contiguous():
-                s[i] = width
-            elif t.dim() == 2 and t.stride(1) == 1:
-                s[i] = t.stride(0)
-            else:
-                raise NebulaError(1, "norm: rows are contiguous, and evenly spaced in two dimensions")
-            a[i] = t.data_ptr()
-        w = [0] * 5
-        for i, t in enumerate((weight, bias, channel_scale, next_weight, next_bias)):
-            if t is None:
-                continue
-            if t.dtype != torch.float32 or t.numel() != width or not t.is_contiguous() or t.device != x.device:
-                raise NebulaError(1, "norm: weights are contiguous float32 tensors of the row's width")
-            w[i] = t.data_ptr()
-        rkind = kinds.get(out.dtype, -1)
-        desc, io = bytearray(_NORM_DESC.size), bytearray(_NORM_IO.size)
-        _NORM_DESC.pack_into(desc, 0, rows, width, groups, NORMS[norm], NORMS[next_norm], GATES[gate_act] if gate is not None else 0, kind,
-                             rkind, eps, scale, *s)
-        _NORM_IO.pack_into(io, 0, a[0], w[0], w[1], a[1], w[2], a[2], a[3], w[3], w[4], a[4])
-        self.check(self.lib.nb_norm_gate_residual(self.h, (C.c_char * len(desc)).from_buffer(desc), (C.c_char * len(io)).from_buffer(io)))
+            y = _empty_like(x)
+        px, sx = _rows(x, shape, dtype, width)
+        pg, sg = (0, 0) if gate is None else _rows(gate, shape, dtype, width)
+        pr, sr = (0, 0) if residual is None else _rows(residual, shape, residual.dtype, width)
+        po, so = _rows(out, shape, like.dtype, width)
+        py, sy = (0, 0) if y is None else _rows(y, shape, dtype, width)
+        _NORM_DESC.pack_into(self._norm_desc, 0, x.numel() // width if width else 0, width, groups, NORMS[norm], NORMS[next_norm],
+                             GATES[gate_act] if gate is not None else 0, kind, _kind(like.dtype), eps, scale, sx, sg, sr, so, sy)
+        _NORM_IO.pack_into(self._norm_io, 0, px, _weights(weight, width), _weights(bias, width), pg, _weights(channel_scale, width), pr, po,
+                           _weights(next_weight, width), _weights(next_bias, width), py)
+        rc = self.lib.nb_norm_gate_residual(self.h, self._norm_desc, self._norm_io)
+        if rc:
+            self.check(rc)
         return out, y
 
     def gemm(self, ta, tb, M, N, K, alpha, A, lda, B, ldb, beta, Cm, ldc):
@@ -510,74 +530,77 @@ class LinearAttention(_Plan):
         self.desc = LinearAttentionDesc(batch, time_steps, heads, key_heads or heads, key_dim, value_dim, DTYPES[dtype], scale)
         handle.check(handle.lib.nb_linear_attention_plan_create(handle.h, C.byref(self.desc), C.byref(self.p)))
         self.dtype = torch.float32 if dtype == "f32" else torch.bfloat16
-        self._key, self._value = (self.desc.key_heads, key_dim), (heads, value_dim)
+        _kind(self.dtype)
         self._state = (heads, key_dim, value_dim)
+        self._whole = self._shapes((batch, time_steps))
+        self._single = self._shapes((batch,))
         self._io = (C.c_char * _ATTENTION_IO.size)()
 
-    def _view(self, t, lead, tail, what):
-        """Address and strides (batch, token, head) of a tensor of tokens."""
-        if t.dtype != self.dtype or t.shape[:-2] != lead or tuple(t.shape[-2:]) != tail or (tail[1] > 1 and t.stride(-1) != 1) or not t.is_cuda:
-            raise NebulaError(1, f"linear attention: {what} is {tuple(t.shape)} {t.dtype} with last stride {t.stride(-1)}, expected "
-                                 f"{(*lead, *tail)} {self.dtype} on the device with contiguous head vectors")
-        st = t.stride()
-        if len(lead) == 2:
-            return t.data_ptr(), st[0], st[1], st[2]
-        return t.data_ptr(), st[0], st[0], st[1]
+    def _shapes(self, lead):
+        """Of q and k, of v and the result, of the log decays."""
+        heads, key_dim, value_dim = self._state
+        return (*lead, self.desc.key_heads, key_dim), (*lead, heads, value_dim), (*lead, heads)
 
-    def _decay(self, g, lead):
+    def _view(self, t, shape, what):
+        """Address and strides (batch, token, head) of a tensor of tokens."""
+        if t.shape == shape and t.dtype is self.dtype and t.is_cuda:
+            st = t.stride()
+            if st[-1] == 1 or shape[-1] == 1:
+                return (t.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (t.data_ptr(), st[0], st[0], st[1])
+        raise NebulaError(1, f"linear attention: {what} is {tuple(t.shape)} {t.dtype} with strides {t.stride()}, expected {shape} {self.dtype} on "
+                             "the device with contiguous head vectors")
+
+    def _decay(self, g, shape):
         if g is None:
             return 0, 0, 0, 0
-        if str(g.dtype) != "torch.float32" or not g.is_cuda or g.shape[-1] != self._value[0] or (g.dim() > 1 and g.shape[:-1] != lead):
-            raise NebulaError(1, f"linear attention: log_decay is {tuple(g.shape)} {g.dtype}, expected float32 {(*lead, self._value[0])} or "
-                                 f"{(self._value[0],)} on the device")
-        st = g.stride()
-        if g.dim() == 1:
-            return g.data_ptr(), 0, 0, st[0]
-        if len(lead) == 2:
-            return g.data_ptr(), st[0], st[1], st[2]
-        return g.data_ptr(), st[0], st[0], st[1]
+        if g.dtype is _torch.float32 and g.is_cuda:
+            if g.shape == shape:
+                st = g.stride()
+                return (g.data_ptr(), st[0], st[1], st[2]) if len(st) == 3 else (g.data_ptr(), st[0], st[0], st[1])
+            if g.shape == shape[-1:]:
+                return g.data_ptr(), 0, 0, g.stride(0)
+        raise NebulaError(1, f"linear attention: log_decay is {tuple(g.shape)} {g.dtype}, expected float32 {shape} or {shape[-1:]} on the device")
 
     def _ints(self, t, n, what):
         if t is None:
             return 0
-        if str(t.dtype) != "torch.int32" or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
+        if t.dtype is not _torch.int32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
             raise NebulaError(1, f"linear attention: {what} is a contiguous int32 tensor of {n} values on the device")
         return t.data_ptr()
 
     def _pool(self, t, slots, what):
         if t is None:
             return 0
-        if str(t.dtype) != "torch.float32" or tuple(t.shape[1:]) != self._state or t.shape[0] != slots or not t.is_contiguous() or not t.is_cuda:
+        if t.dtype is not _torch.float32 or t.shape != (slots, *self._state) or not t.is_contiguous() or not t.is_cuda:
             raise NebulaError(1, f"linear attention: {what} is a contiguous float32 tensor {(slots, *self._state)} on the device")
         return t.data_ptr()
 
-    def _run(self, fn, lead, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out):
-        import torch
+    def _run(self, fn, shapes, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out):
+        keys, values, decays = shapes
         if out is None:
-            out = torch.empty((*lead, *self._value), device=v.device, dtype=self.dtype)
+            out = _torch.empty(values, device=v.device, dtype=self.dtype)
         batch = self.desc.batch
         pool = state if state is not None else state_out
         n = pool.shape[0] if pool is not None and slots is not None else batch
         _ATTENTION_IO.pack_into(
-            self._io, 0, *self._view(q, lead, self._key, "q"), *self._view(k, lead, self._key, "k"), *self._view(v, lead, self._value, "v"),
-            *self._decay(log_decay, lead), *self._view(out, lead, self._value, "out"), self._ints(offsets, batch + 1, "offsets"),
-            self._ints(lengths, batch, "lengths"), lead[0] if offsets is not None else 0, self._pool(state, n, "state"),
-            self._pool(state_out, n, "state_out"), self._ints(slots, batch, "slots"), n)
-        self.handle.check(fn(self.p, self._io))
+            self._io, 0, *self._view(q, keys, "q"), *self._view(k, keys, "k"), *self._view(v, values, "v"), *self._decay(log_decay, decays),
+            *self._view(out, values, "out"), self._ints(offsets, batch + 1, "offsets"), self._ints(lengths, batch, "lengths"),
+            values[0] if offsets is not None else 0, self._pool(state, n, "state"), self._pool(state_out, n, "state_out"),
+            self._ints(slots, batch, "slots"), n)
+        rc = fn(self.p, self._io)
+        if rc:
+            self.handle.check(rc)
         return out
 
     def forward(self, q, k, v, log_decay=None, state=None, state_out=None, offsets=None, lengths=None, slots=None, out=None):
         """Prompts.  `state` is read before the first token of a sequence (None: zeros), `state_out` written behind the last
         (None: not kept; it may be `state`)."""
-        lead = v.shape[:-2] if offsets is not None else (self.desc.batch, self.desc.time_steps)
-        if len(lead) != (1 if offsets is not None else 2):
-            raise NebulaError(1, "linear attention: packed tensors are [tokens, heads, size]")
-        return self._run(self.handle.lib.nb_linear_attention_forward, lead, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out)
+        shapes = self._whole if offsets is None else self._shapes((v.shape[0],))
+        return self._run(self.handle.lib.nb_linear_attention_forward, shapes, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out)
 
     def step(self, q, k, v, log_decay=None, state=None, state_out=None, slots=None, out=None):
         """One token of every sequence, tensors [batch, heads, size]; updates `state`, or writes the new one to `state_out`."""
-        return self._run(self.handle.lib.nb_linear_attention_step, (self.desc.batch,), q, k, v, log_decay, state, state_out, None, None,
-                         slots, out)
+        return self._run(self.handle.lib.nb_linear_attention_step, self._single, q, k, v, log_decay, state, state_out, None, None, slots, out)
 
 
 class Network:

@@ -15,13 +15,14 @@ constexpr int RECURRENT_TOKENS = 16;        // prompts of up to so many tokens g
 
 // ------------------------------------------------------------------ single tokens
 // S' = exp(g) S + k v^T and o = scale q^T S'.  Bound by the state, which is read and written once: 8 bytes a value for 5
-// operations.  A CTA takes `cols` columns of one sequence and head: a thread owns one quad (V = 1: one value) of columns of the
-// rows that are congruent to its own, so that a warp's accesses are whole lines, and keeps its part of q^T S' for the columns in
-// registers; the parts are added in the order of the rows.
+// operations.  A CTA takes `cols` columns of one sequence and head: a thread owns a quad (V = 1: one value) of columns
+// of the rows that are congruent to its own, so that rows are whole lines; all of its part of a state of up to 128 rows is asked
+// for at once, before anything else.  Its parts of q^T S' stay in registers, and are added in the order of the rows.
+// Small CTAs end close together: with one for a whole 128 x 128 state, 64 sequences of 16 heads took 25.4 us (5.3 TB/s).
 // The decay is applied as S + expm1(g) S.  exp(g) rounded to fp32 is off by up to 2^-25, the same way at every token of a head with a
 // fixed decay: over a memory of thousands of tokens that adds up to thousands of roundings (a state of 32768 tokens was 3e-4
 // off), while expm1(g) is off by a share of itself.  A decay of zero (expm1 = -1) forgets whatever was there, infinities and NaN too.
-constexpr int STEP_TPB = 256;
+constexpr int STEP_TPB = 128;
 template <class T, int V>
 __global__ void __launch_bounds__(STEP_TPB) linear_attention_step_kernel(LinAttnParams p, int cols, int tiles) {
     grid_begin();
@@ -39,12 +40,32 @@ __global__ void __launch_bounds__(STEP_TPB) linear_attention_step_kernel(LinAttn
     const T *q = (const T *)p.q.p + b * p.q.batch + h / p.group * p.q.head;
     const T *k = (const T *)p.k.p + b * p.k.batch + h / p.group * p.k.head;
     const T *v = (const T *)p.v.p + b * p.v.batch + h * p.v.head;
+    const bool mine = r0 < lanes && col < p.dv && c * V < cols;
+    const long long at = (s.slot * p.H + h) * (long long)p.dk * p.dv + col;
+    const float *S = p.state + at;
+    float *So = p.state_out + at;
+    constexpr int U = 8;                // rows in flight
+    float x[U][V];
+    auto fetch = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int row = r + u * lanes;
+            if (mine && row < p.dk) {
+                if constexpr (V == 4) {
+                    const float4 f = *(const float4 *)(S + (long long)row * p.dv);
+                    x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
+                } else {
+                    x[u][0] = S[(long long)row * p.dv];
+                }
+            }
+        }
+    };
+    fetch(r0);
     for (int i = threadIdx.x; i < p.dk; i += STEP_TPB) {
         qs[i] = to_f32(q[i]) * p.scale;
         ks[i] = to_f32(k[i]);
     }
     const float less = p.g.p ? expm1f(((const float *)p.g.p)[b * p.g.batch + h * p.g.head]) : 0.0f;
-    const bool mine = r0 < lanes && col < p.dv;
     float vv[V], o[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
@@ -52,40 +73,23 @@ __global__ void __launch_bounds__(STEP_TPB) linear_attention_step_kernel(LinAttn
         o[j] = 0.0f;
     }
     __syncthreads();
-    if (mine) {
-        const long long at = (s.slot * p.H + h) * (long long)p.dk * p.dv + col;
-        const float *S = p.state + at;
-        float *So = p.state_out + at;
-        constexpr int U = 8;                // rows in flight
-        for (int r = r0; r < p.dk; r += U * lanes) {
-            float x[U][V];
+    for (int r = r0; r < p.dk;) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int row = r + u * lanes;
-                if (row < p.dk) {
-                    if constexpr (V == 4) {
-                        const float4 f = *(const float4 *)(S + (long long)row * p.dv);
-                        x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
-                    } else {
-                        x[u][0] = S[(long long)row * p.dv];
-                    }
+        for (int u = 0; u < U; u++) {
+            const int row = r + u * lanes;
+            if (mine && row < p.dk) {
+                const float kk = ks[row], qq = qs[row];
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    x[u][j] = fmaf(kk, vv[j], less == -1.0f ? 0.0f : fmaf(less, x[u][j], x[u][j]));
+                    o[j] = fmaf(qq, x[u][j], o[j]);
                 }
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int row = r + u * lanes;
-                if (row < p.dk) {
-                    const float kk = ks[row], qq = qs[row];
-#pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        x[u][j] = fmaf(kk, vv[j], less == -1.0f ? 0.0f : fmaf(less, x[u][j], x[u][j]));
-                        o[j] = fmaf(qq, x[u][j], o[j]);
-                    }
-                    if constexpr (V == 4) *(float4 *)(So + (long long)row * p.dv) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
-                    else So[(long long)row * p.dv] = x[u][0];
-                }
+                if constexpr (V == 4) *(float4 *)(So + (long long)row * p.dv) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+                else So[(long long)row * p.dv] = x[u][0];
             }
         }
+        r += U * lanes;
+        if (r < p.dk) fetch(r);
     }
 #pragma unroll
     for (int j = 0; j < V; j++) part[j * STEP_TPB + threadIdx.x] = o[j];
@@ -185,10 +189,15 @@ void launch_recurrent(nb_handle_s *h, const LinAttnParams &p) {
 template <class T>
 void launch_step(nb_handle_s *h, const LinAttnParams &p) {
     const bool quads = p.dv % 4 == 0 && ((uintptr_t)p.state | (uintptr_t)p.state_out) % 16 == 0;
-    // whole rows of the state where there are CTAs enough for two per SM; fewer columns, down to 16, where there are not
-    int cols = quads ? 16 : 32;
-    while (cols < p.dv && cols < (quads ? 128 : 256)) cols *= 2;
-    while (cols > 16 && (long long)p.B * p.H * ((p.dv + cols - 1) / cols) < 2 * h->sm_count) cols /= 2;
+    // Columns of a CTA: about 4096 values of the state, a quad of eight rows for each thread; 16 KB is little enough for CTAs to end
+    // together (see the kernel), and enough to hide a CTA's start (in 8 KB pieces states of 64 x 96 took 41.6 us for 333 sequences of
+    // 12 heads).  Never less than 16 columns, and down to that while there are fewer CTAs than SMs.
+    const int unit = quads ? 4 : 1;
+    auto columns = [&](int n) { return std::max(16, (p.dv + n * unit - 1) / (n * unit) * unit); };
+    int n = std::max(1, (int)((long long)p.dk * p.dv + 2048) / 4096);
+    while (columns(n) > (quads ? 128 : 64)) n++;
+    while (columns(n) > 16 && (long long)p.B * p.H * n < h->sm_count) n++;
+    const int cols = columns(n);
     const int tiles = (p.dv + cols - 1) / cols;
     const dim3 grid((unsigned)(p.B * p.H * tiles));
     if (quads) launch_overlapped(h, linear_attention_step_kernel<T, 4>, grid, STEP_TPB, 0, p, cols, tiles);

@@ -8,6 +8,9 @@
 // before it is rounded for storage.
 #include <cuda_bf16.h>
 
+#include <numeric>
+#include <type_traits>
+
 #include "device_math.cuh"
 #include "nb_internal.h"
 
@@ -24,14 +27,23 @@ struct NormParams {
     int width, groups;          // of a row; groups > 1 only in the general kernel
     int fold;                   // > 0: a row here is one of `fold` groups of a row of the tensors
     int norm, next_norm, gate_mode;
-    float eps, scale;
+    float eps, scale, by_width, by_group;       // by_...: 1 / the values of a row, of a group
     int lanes;                  // threads of a row, a power of two
 };
 
+// The logistic function by the hardware's exponential and reciprocal, good to 2^-21 for arguments of ordinary size: with the
+// library's, the norm of 16384 x 16 heads of 128 with a gate waited for arithmetic.
 __device__ __forceinline__ float gate_value(float z, int mode) {
     if (mode == NB_GATE_LINEAR) return z;
-    const float s = 1.0f / (1.0f + expf(-z));
+    float s;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + __expf(-z)));
     return mode == NB_GATE_SIGMOID ? s : z * s;
+}
+// 1 / sqrt(x): the hardware's approximation and a step of Newton's iteration.  (x = 0 and infinity stay what they are.)
+__device__ __forceinline__ float inverse_root(float x) {
+    const float y = rsqrtf(x);
+    const float z = fmaf(fmaf(-x * y, y, 1.0f), 0.5f * y, y);
+    return x > 1e-30f && x < 1e30f ? z : y;
 }
 
 template <class T, int V> struct Raw;
@@ -62,6 +74,12 @@ template <class T, int V> __device__ __forceinline__ void put(void *p, long long
         *(uint4 *)((__nv_bfloat16 *)p + at) = r;
     }
 }
+// a load that stays where it is written (the compiler would keep a loop's biases in registers instead, and fewer rows in flight)
+__device__ __forceinline__ float load_now(const float *p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
 template <int V> __device__ __forceinline__ void weights_at(const float *w, int at, float *f) {
     if constexpr (V == 1) f[0] = w[at];
     else
@@ -73,14 +91,14 @@ template <int V> __device__ __forceinline__ void weights_at(const float *w, int 
 }
 
 // Sum over the threads of a row, the same for all of them.  Rows of up to a warp are segments of one; wider ones are a CTA of their
-// own, whose warps' sums are added in order.
-__device__ __forceinline__ float row_sum(float v, int lanes, float *red) {
+// own, whose warps' sums are added in order.  `red` has a half for each of two sums in turn, so that one barrier a sum is enough.
+__device__ __forceinline__ float row_sum(float v, int lanes, float *red, int &turn) {
     for (int o = min(lanes, 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lanes <= 32) return v;
-    __syncthreads();            // the sums of the call before have been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    float *r = red + (turn ^= 32);
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (threadIdx.x & 31) < (lanes >> 5) ? red[threadIdx.x & 31] : 0.0f;
+    v = (threadIdx.x & 31) < (lanes >> 5) ? r[threadIdx.x & 31] : 0.0f;
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
@@ -107,29 +125,177 @@ __device__ __forceinline__ void group_sums(const NormParams &p, float *parts, fl
 }
 
 // T: type of x, gate and y.  R: type of residual and s.  V: values of one access.  NV: accesses of a thread.
-// GROUPED: several groups a row (the first norm), for rows that a second norm joins again.
-template <class T, class R, int V, int NV, bool GROUPED>
+
+// Rows of at most 256 threads, which is where the time goes.  A CTA takes rows in turn and asks for the next one's values before it
+// works on this one's.  A thread has the same columns of every row (launch_rows sees to it where rows are groups of the tensors'), so
+// that addresses are steps of 32 bits; the weights, the block's scales multiplied in, lie in shared memory (in registers they leave
+// room for too few rows in flight: 8192 rows of 4096 took 81 us).  With weights loaded from L1 and addresses worked out for every
+// row, 48 instructions were issued a value: 66 us, and 16384 x 16 x 128 with a gate 72.
+template <class T, class R, int V, int NV, bool GATE>
+__global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
+    grid_begin();
+    // the weights of both norms for a row of the tensors, four values of every vector after four of every vector
+    extern __shared__ __align__(16) float smem[];
+    __shared__ float red[64];
+    const int lane = threadIdx.x & (p.lanes - 1), per_cta = blockDim.x / p.lanes;
+    int turn = 0;
+    const long long row0 = (long long)blockIdx.x * per_cta + threadIdx.x / p.lanes, pace = (long long)gridDim.x * per_cta;
+    const int fold = max(p.fold, 1), first = (int)(row0 % fold) * p.width;
+    const unsigned r0 = (unsigned)(row0 / fold), step = (unsigned)(pace / fold);
+    unsigned ox = r0 * (unsigned)p.x_stride + first, og = r0 * (unsigned)p.gate_stride + first, orr = r0 * (unsigned)p.residual_stride + first,
+             os = r0 * (unsigned)p.sum_stride + first, oy = r0 * (unsigned)p.y_stride + first;
+    const unsigned dx = step * (unsigned)p.x_stride, dg = step * (unsigned)p.gate_stride, dr = step * (unsigned)p.residual_stride,
+                   ds = step * (unsigned)p.sum_stride, dy = step * (unsigned)p.y_stride;
+    bool in[NV];
+#pragma unroll
+    for (int n = 0; n < NV; n++) in[n] = (n * p.lanes + lane) * V < p.width;
+    constexpr int Q = V == 1 ? 1 : 4;
+    const int total = fold * p.width, vecs = total / V;
+    for (int i = threadIdx.x; i < total; i += blockDim.x) {
+        const int to = V == 1 ? i : (i % V / Q * vecs + i / V) * Q + i % Q;
+        smem[to] = (p.weight ? p.weight[i] : 1.0f) * (p.channel_scale ? p.scale * p.channel_scale[i] : p.scale);
+        if (p.next_weight) smem[total + to] = p.next_weight[i];
+    }
+    __syncthreads();
+    // f *= by * weights
+    auto weigh = [&](float (&f)[V], const float *weights, int n, float by) {
+        const float *w = weights + (first / V + n * p.lanes + lane) * Q;
+#pragma unroll
+        for (int i = 0; i < V; i += Q) {
+            if constexpr (V == 1) {
+                f[0] *= by * w[0];
+            } else {
+                const float4 v = *(const float4 *)(w + i / Q * vecs * Q);
+                f[i] *= by * v.x;
+                f[i + 1] *= by * v.y;
+                f[i + 2] *= by * v.z;
+                f[i + 3] *= by * v.w;
+            }
+        }
+    };
+    Raw<T, V> x[NV], gate[GATE ? NV : 1];
+    Raw<R, V> res[NV];
+    auto ask = [&](bool live) {
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            const unsigned c = (unsigned)((n * p.lanes + lane) * V);
+            x[n] = {};
+            res[n] = {};
+            if (live && in[n]) {
+                x[n] = fetch<T, V>(p.x, ox + c);
+                if constexpr (GATE) gate[n] = fetch<T, V>(p.gate, og + c);
+                if (p.residual) res[n] = fetch<R, V>(p.residual, orr + c);
+            }
+        }
+    };
+    // of a row's values, subtracts the mean (of the layer norm) and returns 1 / the root of the mean square
+    auto spread = [&](float (&f)[NV][V], int mode) {
+        if (mode == NB_NORM_LAYER) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+#pragma unroll
+                for (int i = 0; i < V; i++) sum += f[n][i];         // (columns past the last are zeros)
+            const float mean = row_sum(sum, p.lanes, red, turn) * p.by_width;
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+                if (in[n])
+#pragma unroll
+                    for (int i = 0; i < V; i++) f[n][i] -= mean;
+        }
+        float power = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+#pragma unroll
+            for (int i = 0; i < V; i++) power = fmaf(f[n][i], f[n][i], power);
+        return inverse_root(fmaf(row_sum(power, p.lanes, red, turn), p.by_width, p.eps));
+    };
+    ask(row0 < p.rows);
+    long long row = row0;
+    for (long long base = (long long)blockIdx.x * per_cta; base < p.rows; base += pace) {
+        const bool live = row < p.rows;
+        float f[NV][V];
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+#pragma unroll
+            for (int i = 0; i < V; i++) f[n][i] = x[n].get(i);
+        Raw<T, V> z[GATE ? NV : 1];
+        Raw<R, V> add[NV];
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            if constexpr (GATE) z[n] = gate[n];
+            add[n] = res[n];
+        }
+        row += pace;
+        ox += dx, og += dg, orr += dr;
+        if (base + pace < p.rows) ask(row < p.rows);
+        const float by = p.norm != NB_NORM_NONE ? spread(f, p.norm) : 1.0f;
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            if (!in[n]) continue;
+            const unsigned c = (unsigned)((n * p.lanes + lane) * V);
+            weigh(f[n], smem, n, by);
+            if (p.bias)
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    f[n][i] = fmaf(load_now(p.bias + first + c + i), p.channel_scale ? p.scale * load_now(p.channel_scale + first + c + i) : p.scale, f[n][i]);
+            if constexpr (GATE)
+#pragma unroll
+                for (int i = 0; i < V; i++) f[n][i] *= gate_value(z[n].get(i), p.gate_mode);
+            if (p.residual)
+#pragma unroll
+                for (int i = 0; i < V; i++) f[n][i] += add[n].get(i);
+            if (p.sum && live) put<R, V>(p.sum, os + c, f[n]);
+        }
+        os += ds;
+        if (p.next_norm != NB_NORM_NONE) {
+            const float by2 = spread(f, p.next_norm);
+#pragma unroll
+            for (int n = 0; n < NV; n++) {
+                if (!in[n]) continue;
+                const unsigned c = (unsigned)((n * p.lanes + lane) * V);
+                if (p.next_weight) {
+                    weigh(f[n], smem + total, n, by2);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++) f[n][i] *= by2;
+                }
+                if (p.next_bias)
+#pragma unroll
+                    for (int i = 0; i < V; i++) f[n][i] += load_now(p.next_bias + first + c + i);
+                if (live) put<T, V>(p.y, oy + c, f[n]);
+            }
+        }
+        oy += dy;
+    }
+}
+
+// The others: wide rows, rows whose groups a second norm joins (GROUPED), tensors of more than 2^32 values.  GATE: there is a gate.
+template <class T, class R, int V, int NV, bool GROUPED, bool GATE>
 __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
     grid_begin();
     extern __shared__ float smem[];         // GROUPED: a value per vector of the row, then one per group
-    __shared__ float red[32];
+    __shared__ float red[64];
     const int lane = threadIdx.x & (p.lanes - 1);
+    int turn = 0;
     const long long row = (long long)blockIdx.x * (blockDim.x / p.lanes) + threadIdx.x / p.lanes;
     const bool live = row < p.rows;
     const long long r = p.fold ? row / p.fold : row;
-    const int first = p.fold ? (int)(row % p.fold) * p.width : 0;
+    const int first = p.fold ? (int)(row - r * p.fold) * p.width : 0;
     float f[NV * V];
-    Raw<T, V> gate[NV];
+    Raw<T, V> gate[GATE ? NV : 1];
     Raw<R, V> res[NV];
 #pragma unroll
     for (int n = 0; n < NV; n++) {
         const int c = (n * p.lanes + lane) * V;
         const bool in = live && c < p.width;
         Raw<T, V> x = {};
-        gate[n] = {};
         res[n] = {};
         if (in) x = fetch<T, V>(p.x, r * p.x_stride + first + c);
-        if (in && p.gate) gate[n] = fetch<T, V>(p.gate, r * p.gate_stride + first + c);
+        if constexpr (GATE) {
+            gate[n] = {};
+            if (in) gate[n] = fetch<T, V>(p.gate, r * p.gate_stride + first + c);
+        }
         if (in && p.residual) res[n] = fetch<R, V>(p.residual, r * p.residual_stride + first + c);
 #pragma unroll
         for (int i = 0; i < V; i++) f[n * V + i] = x.get(i);
@@ -141,7 +307,7 @@ __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV * V; i++) sum += f[i];
-            mean = row_sum(sum, p.lanes, red) / p.width;
+            mean = row_sum(sum, p.lanes, red, turn) * p.by_width;
         }
         float power = 0.0f;
 #pragma unroll
@@ -152,7 +318,7 @@ __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
                     f[n * V + i] -= mean;
                     power = fmaf(f[n * V + i], f[n * V + i], power);
                 }
-        const float by = 1.0f / sqrtf(row_sum(power, p.lanes, red) / p.width + p.eps);
+        const float by = inverse_root(fmaf(row_sum(power, p.lanes, red, turn), p.by_width, p.eps));
 #pragma unroll
         for (int i = 0; i < NV * V; i++) f[i] *= by;
     };
@@ -170,7 +336,7 @@ __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
 #pragma unroll
                 for (int n = 0; n < NV; n++)
                     if (inside(n)) {
-                        const float mean = sums[(n * p.lanes + lane) * V / per] / per;
+                        const float mean = sums[(n * p.lanes + lane) * V / per] * p.by_group;
 #pragma unroll
                         for (int i = 0; i < V; i++) f[n * V + i] -= mean;
                     }
@@ -184,7 +350,7 @@ __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
 #pragma unroll
             for (int n = 0; n < NV; n++)
                 if (inside(n)) {
-                    const float by = 1.0f / sqrtf(sums[(n * p.lanes + lane) * V / per] / per + p.eps);
+                    const float by = inverse_root(fmaf(sums[(n * p.lanes + lane) * V / per], p.by_group, p.eps));
 #pragma unroll
                     for (int i = 0; i < V; i++) f[n * V + i] *= by;
                 }
@@ -207,7 +373,7 @@ __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
 #pragma unroll
                 for (int i = 0; i < V; i++) f[n * V + i] += w[i];
             }
-            if (p.gate)
+            if constexpr (GATE)
 #pragma unroll
                 for (int i = 0; i < V; i++) f[n * V + i] *= gate_value(gate[n].get(i), p.gate_mode);
             if (p.channel_scale) {
@@ -242,43 +408,74 @@ __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
     }
 }
 
-template <class T, class R, int V, int NV>
-void launch_norm(nb_handle_s *h, const NormParams &p) {
+template <class T, class R, int V, int NV, bool GROUPED, bool GATE>
+void launch_general(nb_handle_s *h, const NormParams &p) {
+    auto kernel = norm_gate_kernel<T, R, V, NV, GROUPED, GATE>;
     const int tpb = p.lanes > 32 ? p.lanes : 128;      // a row of more than a warp has a CTA of its own
-    const dim3 grid((unsigned)((p.rows + tpb / p.lanes - 1) / (tpb / p.lanes)));
-    const size_t smem = p.groups > 1 ? (size_t)(p.width / V + p.groups) * sizeof(float) : 0;
-    NB_REQUIRE((p.rows + tpb / p.lanes - 1) / (tpb / p.lanes) < (1LL << 31), "norm: too many rows");
-    if (p.groups > 1) {
-        if (smem > 200 * 1024) throw Error(NB_ERR_UNSUPPORTED, "norm: too many groups in a row of this width");
-        if (smem > 48 * 1024)
-            NB_CHECK_CUDA(cudaFuncSetAttribute(norm_gate_kernel<T, R, V, NV, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        launch_overlapped(h, norm_gate_kernel<T, R, V, NV, true>, grid, tpb, smem, p);
-    } else {
-        launch_overlapped(h, norm_gate_kernel<T, R, V, NV, false>, grid, tpb, 0, p);
-    }
+    const long long ctas = (p.rows + tpb / p.lanes - 1) / (tpb / p.lanes);
+    NB_REQUIRE(ctas < (1LL << 31), "norm: too many rows");
+    const size_t smem = GROUPED ? (size_t)(p.width / V + p.groups) * sizeof(float) : 0;
+    if (smem > 200 * 1024) throw Error(NB_ERR_UNSUPPORTED, "norm: too many groups in a row of this width");
+    if (smem > 48 * 1024) NB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    launch_overlapped(h, kernel, dim3((unsigned)ctas), tpb, smem, p);
     check_launch("norm_gate_kernel");
     count_launch(h);
 }
 
+// Returns false where the threads' columns cannot be the same in all rows of theirs.
+template <class T, class R, int V, int NV, bool GATE>
+bool launch_rows(nb_handle_s *h, const NormParams &p) {
+    auto kernel = norm_gate_rows_kernel<T, R, V, NV, GATE>;
+    const int tpb = p.lanes > 32 ? p.lanes : 256, per_cta = tpb / p.lanes;
+    const int total = std::max(p.fold, 1) * p.width;
+    const size_t smem = (size_t)total * (p.next_weight ? 2 : 1) * sizeof(float);
+    if (smem > 48 * 1024) return false;
+    const long long ctas = (p.rows + per_cta - 1) / per_cta;
+    // (what the device holds at once: 80 registers a thread and the shared memory)
+    const int resident = std::max(1, std::min(768 / tpb, (int)(200 * 1024 / (smem + 2048))));
+    long long grid = std::min<long long>(ctas, (long long)resident * h->sm_count);
+    if (p.fold && grid < ctas) {            // a step of the grid is a whole number of the tensors' rows
+        const long long unit = p.fold / std::gcd(p.fold, per_cta);
+        if (grid < unit) return false;
+        grid -= grid % unit;
+    }
+    launch_overlapped(h, kernel, dim3((unsigned)grid), tpb, smem, p);
+    check_launch("norm_gate_rows_kernel");
+    count_launch(h);
+    return true;
+}
+
 constexpr int MAX_WIDTH = 32768;        // 1024 threads with 32 values each
 
-// Threads and accesses of a row: as few threads as hold it with `most` accesses each, but rather more threads than a second
-// access while the rows are fewer than the device's SMs.
+// Threads and accesses of a row: two accesses a thread, or one while the rows are too few to fill the device and a row's
+// latency counts; more where 1024 threads do not hold it.  wide: offsets need 64 bits.
 template <class T, class R, int V>
-void choose(nb_handle_s *h, NormParams p, int most) {
+void choose(nb_handle_s *h, NormParams p, bool wide) {
     const int vecs = (p.width + V - 1) / V;
-    const int want = p.rows * 2 <= h->sm_count ? 1 : std::min(2, most);
+    const int want = p.rows * 2 <= h->sm_count ? 1 : 2;
     int lanes = p.groups > 1 ? 64 : 4;
     while (lanes < 1024 && lanes * want < vecs) lanes *= 2;
     p.lanes = lanes;
     const int nv = (vecs + lanes - 1) / lanes;
-    if (nv <= 1) launch_norm<T, R, V, 1>(h, p);
-    else if (nv <= 2) launch_norm<T, R, V, 2>(h, p);
-    else if (nv <= 4) launch_norm<T, R, V, 4>(h, p);
-    else if constexpr (V < 8) {
-        if (nv <= 8) launch_norm<T, R, V, 8>(h, p);
-        else if constexpr (V == 1) launch_norm<T, R, V, 32>(h, p);
+    if (p.groups == 1 && lanes <= 256 && nv <= 2 && !wide) {
+        const bool done = nv <= 1 ? p.gate ? launch_rows<T, R, V, 1, true>(h, p) : launch_rows<T, R, V, 1, false>(h, p)
+                                  : p.gate ? launch_rows<T, R, V, 2, true>(h, p) : launch_rows<T, R, V, 2, false>(h, p);
+        if (done) return;
     }
+    auto go = [&](auto accesses) {
+        constexpr int NV = decltype(accesses)::value;
+        if (p.groups > 1) {
+            if (p.gate) launch_general<T, R, V, NV, true, true>(h, p);
+            else launch_general<T, R, V, NV, true, false>(h, p);
+        } else {
+            if (p.gate) launch_general<T, R, V, NV, false, true>(h, p);
+            else launch_general<T, R, V, NV, false, false>(h, p);
+        }
+    };
+    if (nv <= 2) go(std::integral_constant<int, 2>());
+    else if constexpr (V == 8) go(std::integral_constant<int, 4>());
+    else if constexpr (V == 4) go(std::integral_constant<int, 8>());
+    else go(std::integral_constant<int, 32>());
 }
 
 }  // namespace
@@ -300,6 +497,7 @@ void launch_norm_gate(nb_handle_s *h, const nb_norm_gate_desc_t &d, const nb_nor
     const size_t tb = d.dtype == NB_DTYPE_BF16 ? 2 : 4, rb = d.residual_dtype == NB_DTYPE_BF16 ? 2 : 4;
     NormParams p = {};
     size_t align = 0;           // addresses and strides in bytes, or-ed
+    bool wide = false;          // some tensor has values past the 2^32nd
     auto rows = [&](const void *ptr, long long stride, size_t bytes, const char *what) {
         const long long s = stride ? stride : d.width;
         if (!ptr) return s;
@@ -307,6 +505,7 @@ void launch_norm_gate(nb_handle_s *h, const nb_norm_gate_desc_t &d, const nb_nor
         NB_REQUIRE((uintptr_t)ptr % bytes == 0, std::string("norm: misaligned ") + what);
         check_extent(h, ptr, 0, ((d.rows - 1) * s + d.width) * (long long)bytes, what);
         align |= (uintptr_t)ptr | (size_t)(s * (long long)bytes);
+        wide = wide || (d.rows - 1) * s + d.width >= (1LL << 32);
         return s;
     };
     p.x_stride = rows(io.x, d.x_stride, tb, "x");
@@ -330,18 +529,20 @@ void launch_norm_gate(nb_handle_s *h, const nb_norm_gate_desc_t &d, const nb_nor
         p.width /= p.groups;
         p.groups = 1;
     }
+    p.by_width = 1.0f / p.width;
+    p.by_group = (float)p.groups / p.width;
     // whole accesses of 16 bytes: every row, group and vector of weights starts on such a boundary and is made of whole ones
     const int v = d.dtype == NB_DTYPE_BF16 ? 8 : 4;
     const bool whole = align % 16 == 0 && p.width % v == 0 && p.width / p.groups % v == 0;
     if (d.dtype == NB_DTYPE_F32) {
-        if (whole) choose<float, float, 4>(h, p, 8);
-        else choose<float, float, 1>(h, p, 32);
+        if (whole) choose<float, float, 4>(h, p, wide);
+        else choose<float, float, 1>(h, p, wide);
     } else if (d.residual_dtype == NB_DTYPE_BF16) {
-        if (whole) choose<__nv_bfloat16, __nv_bfloat16, 8>(h, p, 4);
-        else choose<__nv_bfloat16, __nv_bfloat16, 1>(h, p, 32);
+        if (whole) choose<__nv_bfloat16, __nv_bfloat16, 8>(h, p, wide);
+        else choose<__nv_bfloat16, __nv_bfloat16, 1>(h, p, wide);
     } else {
-        if (whole) choose<__nv_bfloat16, float, 8>(h, p, 4);
-        else choose<__nv_bfloat16, float, 1>(h, p, 32);
+        if (whole) choose<__nv_bfloat16, float, 8>(h, p, wide);
+        else choose<__nv_bfloat16, float, 1>(h, p, wide);
     }
 }
 
