@@ -107,13 +107,19 @@ __global__ void __launch_bounds__(STEP_TPB) linear_attention_step_kernel(LinAttn
 // shared memory; queries and keys are read from there as broadcasts.  Bound by the chain of tokens.
 constexpr int REC_TPB = 128, REC_TOK = 16, REC_COLS = 32;
 template <class T, int KR>
-__global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(LinAttnParams p, int tiles) {
+__global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(LinAttnParams p, int tiles, const int *odd, int chunks, const float *ws) {
     grid_begin();
     __shared__ __align__(16) float qs[REC_TOK][4 * KR], ks[REC_TOK][4 * KR];
     __shared__ float vs[REC_TOK][REC_COLS], part[4][REC_TOK][REC_COLS], ds[REC_TOK];
     const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % p.H, b = bh / p.H;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = tile * REC_COLS + lane;
     const SeqAt s = seq_at(p, b);
+    if (odd) {                  // a repair
+        int any = 0;
+        if (s.slot >= 0)
+            for (int c = threadIdx.x; c * 64 < s.len; c += REC_TPB) any |= odd[bh * chunks + c];
+        if (!__syncthreads_or(any)) return;
+    }
     const T *q = (const T *)p.q.p + token_base(p, p.q, b, s, h / p.group), *k = (const T *)p.k.p + token_base(p, p.k, b, s, h / p.group);
     const T *v = (const T *)p.v.p + token_base(p, p.v, b, s, h);
     const float *g = p.g.p ? (const float *)p.g.p + token_base(p, p.g, b, s, h) : nullptr;
@@ -128,7 +134,8 @@ __global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(Lin
 #pragma unroll
     for (int i = 0; i < KR; i++) {
         const int row = warp * KR + i;
-        S[i] = p.state && row < p.dk && col < p.dv ? p.state[at + (long long)row * p.dv] : 0.0f;
+        const float *from = odd ? ws + (long long)bh * chunks * p.dk * p.dv + col : p.state ? p.state + at : nullptr;
+        S[i] = from && row < p.dk && col < p.dv ? from[(long long)row * p.dv] : 0.0f;
     }
     for (int t0 = 0; t0 < s.len; t0 += REC_TOK) {
         const int n = min(REC_TOK, s.len - t0);
@@ -174,14 +181,15 @@ __global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(Lin
 }
 
 template <class T>
-void launch_recurrent(nb_handle_s *h, const LinAttnParams &p) {
+void launch_recurrent(nb_handle_s *h, const LinAttnParams &p, const int *odd = nullptr, int chunks = 0, const float *ws = nullptr) {
     const int tiles = (p.dv + REC_COLS - 1) / REC_COLS;
     const dim3 grid((unsigned)(p.B * p.H * tiles));
-    if (p.dk <= 16) launch_overlapped(h, linear_attention_recurrent_kernel<T, 4>, grid, REC_TPB, 0, p, tiles);
-    else if (p.dk <= 32) launch_overlapped(h, linear_attention_recurrent_kernel<T, 8>, grid, REC_TPB, 0, p, tiles);
-    else if (p.dk <= 64) launch_overlapped(h, linear_attention_recurrent_kernel<T, 16>, grid, REC_TPB, 0, p, tiles);
-    else if (p.dk <= 128) launch_overlapped(h, linear_attention_recurrent_kernel<T, 32>, grid, REC_TPB, 0, p, tiles);
-    else launch_overlapped(h, linear_attention_recurrent_kernel<T, 64>, grid, REC_TPB, 0, p, tiles);
+    auto go = [&](auto kernel) { launch_overlapped(h, kernel, grid, REC_TPB, 0, p, tiles, odd, chunks, ws); };
+    if (p.dk <= 16) go(linear_attention_recurrent_kernel<T, 4>);
+    else if (p.dk <= 32) go(linear_attention_recurrent_kernel<T, 8>);
+    else if (p.dk <= 64) go(linear_attention_recurrent_kernel<T, 16>);
+    else if (p.dk <= 128) go(linear_attention_recurrent_kernel<T, 32>);
+    else go(linear_attention_recurrent_kernel<T, 64>);
     check_launch("linear_attention_recurrent_kernel");
     count_launch(h);
 }
@@ -208,6 +216,11 @@ void launch_step(nb_handle_s *h, const LinAttnParams &p) {
 
 }  // namespace
 
+void linear_attention_repair(nb_handle_s *h, const LinAttnParams &p, bool bf16, const int *odd, int chunks, const float *ws) {
+    if (bf16) launch_recurrent<__nv_bfloat16>(h, p, odd, chunks, ws);
+    else launch_recurrent<float>(h, p, odd, chunks, ws);
+}
+
 LinAttnPlan::LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc) : nb_plan_s(NB_PLAN_LINEAR_ATTENTION, h), d(desc) {
     NB_REQUIRE(d.batch > 0 && d.time_steps > 0 && d.heads > 0 && d.key_heads > 0, "linear attention: non-positive extent");
     NB_REQUIRE(d.key_dim > 0 && d.value_dim > 0, "linear attention: non-positive head size");
@@ -216,8 +229,10 @@ LinAttnPlan::LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc)
     if (d.key_dim > MAX_DIM || d.value_dim > MAX_DIM) throw Error(NB_ERR_UNSUPPORTED, "linear attention: heads of more than 256 values");
     // grids are indexed in 31 bits, the smallest column tile being 16 wide
     NB_REQUIRE((long long)d.batch * d.heads * ((d.value_dim + 15) / 16) < (1LL << 31), "linear attention: too many sequences and heads");
-    chunked = linear_attention_chunks_supported(d) && d.time_steps > RECURRENT_TOKENS;
-    if (chunked) split = linear_attention_split(d, h->sm_count);
+    route = d.time_steps <= RECURRENT_TOKENS ? TOKENS : linear_attention_chunks_supported(d) ? TENSOR_CORES : CUDA_CORES;
+    if (route == TENSOR_CORES) split = linear_attention_split(d, h->sm_count);
+    if (route == CUDA_CORES)
+        NB_REQUIRE((long long)d.batch * d.heads * ((d.time_steps + 63) / 64) < (1LL << 31), "linear attention: too many tokens");
 }
 
 LinAttnParams LinAttnPlan::params(const nb_linear_attention_io_t &io, bool step) const {
@@ -270,17 +285,17 @@ LinAttnParams LinAttnPlan::params(const nb_linear_attention_io_t &io, bool step)
 }
 
 void LinAttnPlan::reserve() {
-    if (chunked && split.n > 1) ws.reserve(linear_attention_workspace(d, split));
+    if (route == TENSOR_CORES && split.n > 1) ws.reserve(linear_attention_workspace(d, split));
+    if (route == CUDA_CORES) ws.reserve(linear_attention_simt_workspace(d));
 }
 
 void LinAttnPlan::forward(const nb_linear_attention_io_t &io) {
     const LinAttnParams p = params(io, false);
-    if (chunked) {
-        reserve();
-        linear_attention_chunks(h, p, split, ws.p);
-        return;
-    }
-    if (d.dtype == NB_DTYPE_BF16) launch_recurrent<__nv_bfloat16>(h, p);
+    const bool bf16 = d.dtype == NB_DTYPE_BF16;
+    reserve();
+    if (route == TENSOR_CORES) linear_attention_chunks(h, p, split, ws.p);
+    else if (route == CUDA_CORES) linear_attention_simt(h, p, bf16, ws.p);
+    else if (bf16) launch_recurrent<__nv_bfloat16>(h, p);
     else launch_recurrent<float>(h, p);
 }
 

@@ -1,0 +1,293 @@
+// Linear attention over prompts in chunks of 64 tokens with exact fp32 products on the CUDA cores: fp32 tensors, and heads that
+// the tensor-core kernels do not take.  The chunks are worked on side by side, in three launches:
+//   1. each chunk's own contribution to the state, D_c = sum_j exp(G_end,j) k_j v_j^T, and its decay;
+//   2. the states in front of the chunks, S_{c+1} = exp(G_c) S_c + D_c, every value of a state by one thread;
+//   3. out_i = scale * [ sum_{j<=i} exp(G_ij) (q_i . k_j) v_j + exp(G_i) q_i^T S_c ].
+// Bound by fp32 arithmetic (C (dk + dv) + 2 dk dv FMAs a token and head); a thread has 8 x 4 values of a 64 x 64 product, so that
+// three 16-byte reads of shared memory feed 32 FMAs.
+// G, the sums of log decays, are kept to 48 bits (two fp32 numbers), because the weight of two late tokens of a chunk is the
+// difference of two large sums.  A product with a masked weight of zero is NaN where v is not finite: the first launch looks for
+// such values, and the sequences and heads that have any are done once more, token by token.
+#include <algorithm>
+
+#include "device_math.cuh"
+#include "linear_attention.h"
+
+namespace nb {
+
+namespace {
+
+constexpr int C = 64, TPB = 128, PITCH = C + 4;     // 16-byte rows whose starts differ in their banks
+constexpr float RESET = -104.0f;                     // exp of this and less is 0 in fp32
+
+struct SimtParams {
+    LinAttnParams a;
+    int chunks;                 // of the longest sequence
+    float *ws;                  // [B*H][chunks][dk][dv]: contributions, then the states in front of the chunks
+    float *less;                // [B*H][chunks]: expm1 of a chunk's whole log decay, -1 where it holds a reset
+    int *odd;                   // [B*H][chunks]: the chunk's keys or values are not all finite
+};
+
+// Sums of log decays from the chunk's start, resets left out, and the position of each token's last reset.
+struct Sums {
+    float hi[C], lo[C];
+    int since[C];               // 1 + the last token with a reset up to this one, 0: none
+    float total;                // of the chunk
+};
+// By the first warp; two tokens a lane.
+__device__ __forceinline__ void sum_decays(const SimtParams &p, const float *g, int n, Sums &s) {
+    const int lane = threadIdx.x;
+    const float f0 = g && 2 * lane < n ? g[2 * lane * p.a.g.token] : 0.0f, f1 = g && 2 * lane + 1 < n ? g[(2 * lane + 1) * p.a.g.token] : 0.0f;
+    const bool r0 = f0 <= RESET, r1 = f1 <= RESET;
+    const double g0 = r0 ? 0.0 : f0;
+    double up = g0 + (r1 ? 0.0 : f1);
+    int last = r1 ? 2 * lane + 2 : r0 ? 2 * lane + 1 : 0;
+    const double own = up;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, up, o);
+        const int l = __shfl_up_sync(0xffffffffu, last, o);
+        if (lane >= o) {
+            up += u;
+            last = max(last, l);
+        }
+    }
+    const int before = __shfl_up_sync(0xffffffffu, last, 1);
+    const double s0 = up - own + g0;
+    s.hi[2 * lane] = (float)s0;
+    s.lo[2 * lane] = (float)(s0 - (double)(float)s0);
+    s.hi[2 * lane + 1] = (float)up;
+    s.lo[2 * lane + 1] = (float)(up - (double)(float)up);
+    s.since[2 * lane] = r0 ? 2 * lane + 1 : lane ? before : 0;
+    s.since[2 * lane + 1] = last;
+    if (lane == 31) s.total = (float)up;
+}
+// exp of the log decays of tokens j + 1 .. i
+__device__ __forceinline__ float between(const Sums &s, int i, int j) { return s.since[i] > j + 1 ? 0.0f : expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])); }
+
+struct Place {
+    SeqAt s;
+    int b, h, chunk, t0, n;     // n tokens from t0 on
+    bool there;
+};
+__device__ __forceinline__ Place place_of(const SimtParams &p) {
+    Place w;
+    w.chunk = blockIdx.x % p.chunks;
+    const int bh = blockIdx.x / p.chunks;
+    w.h = bh % p.a.H;
+    w.b = bh / p.a.H;
+    w.s = seq_at(p.a, w.b);
+    w.t0 = w.chunk * C;
+    w.n = min(C, w.s.len - w.t0);
+    w.there = w.n > 0;
+    return w;
+}
+
+// 64 x 64 values of a tensor, zeros where there are none: rows = tokens from `src` on, columns from `col` of `width`.
+// TRANSPOSED: [column][token].  Returns what is 0 if all are finite.
+template <class T, bool TRANSPOSED>
+__device__ __forceinline__ float load_tile(float *dst, const T *src, long long token, int n, int col, int width) {
+    float seen = 0.0f;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < C * C; i += TPB) {
+        const int r = i / C, c = i % C;
+        const float v = r < n && col + c < width ? to_f32(src[r * token + col + c]) : 0.0f;
+        seen = fmaf(v, 0.0f, seen);
+        dst[TRANSPOSED ? c * PITCH + r : r * PITCH + c] = v;
+    }
+    return seen;
+}
+// f += A^T B for A [64 k][64 m], B [64 k][64 n] in shared memory; the thread's rows 8 (t / 16).., columns 4 (t % 16)..
+__device__ __forceinline__ void multiply(float (&f)[8][4], const float *A, const float *B) {
+    const float *a = A + threadIdx.x / 16 * 8, *b = B + threadIdx.x % 16 * 4;
+#pragma unroll 8
+    for (int k = 0; k < C; k++) {
+        const float4 x = *(const float4 *)(a + k * PITCH), y = *(const float4 *)(a + k * PITCH + 4), z = *(const float4 *)(b + k * PITCH);
+        const float u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}, v[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[i][j] = fmaf(u[i], v[j], f[i][j]);
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(TPB) linear_attention_contribution_kernel(SimtParams p) {
+    grid_begin();
+    extern __shared__ __align__(16) float smem[];
+    __shared__ Sums sums;
+    float *K = smem, *V = smem + C * PITCH;
+    const Place w = place_of(p);
+    if (!w.there || w.s.slot < 0) return;
+    const LinAttnParams &a = p.a;
+    const T *k = (const T *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group) + w.t0 * a.k.token;
+    const T *v = (const T *)a.v.p + token_base(a, a.v, w.b, w.s, w.h) + w.t0 * a.v.token;
+    if (threadIdx.x < 32) sum_decays(p, a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr, w.n, sums);
+    float *D = p.ws + (size_t)blockIdx.x * a.dk * a.dv;
+    float seen = 0.0f;
+    for (int d0 = 0; d0 < a.dk; d0 += C) {
+        __syncthreads();
+        seen += load_tile<T, false>(K, k, a.k.token, w.n, d0, a.dk);
+        __syncthreads();
+        if (threadIdx.x < C) {                          // the weights go to the keys
+            const float by = between(sums, C - 1, threadIdx.x);
+            for (int c = 0; c < C; c++) K[threadIdx.x * PITCH + c] *= by;
+        }
+        for (int v0 = 0; v0 < a.dv; v0 += C) {
+            __syncthreads();
+            seen += load_tile<T, false>(V, v, a.v.token, w.n, v0, a.dv);
+            __syncthreads();
+            float f[8][4] = {};
+            multiply(f, K, V);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int r = d0 + threadIdx.x / 16 * 8 + i, c = v0 + threadIdx.x % 16 * 4 + j;
+                    if (r < a.dk && c < a.dv) D[(size_t)r * a.dv + c] = f[i][j];
+                }
+        }
+    }
+    const int odd = __syncthreads_or(!(seen == 0.0f));
+    if (threadIdx.x == 0) {
+        p.odd[blockIdx.x] = odd;
+        p.less[blockIdx.x] = sums.since[C - 1] ? -1.0f : expm1f(sums.total);
+    }
+}
+
+// S before each chunk, in place of the chunks' contributions.
+__global__ void __launch_bounds__(256) linear_attention_scan_kernel(SimtParams p, int blocks) {
+    grid_begin();
+    const int bh = blockIdx.x / blocks, h = bh % p.a.H, b = bh / p.a.H;
+    const long long size = (long long)p.a.dk * p.a.dv, i = (long long)(blockIdx.x % blocks) * blockDim.x + threadIdx.x;
+    const SeqAt s = seq_at(p.a, b);
+    if (i >= size || s.slot < 0) return;
+    const long long at = (s.slot * p.a.H + h) * size + i;
+    const int n = (s.len + C - 1) / C;
+    float S = p.a.state ? p.a.state[at] : 0.0f;
+    float *ws = p.ws + (long long)bh * p.chunks * size + i;
+    const float *less = p.less + (long long)bh * p.chunks;
+    constexpr int U = 8;                    // contributions asked for at once
+    for (int c0 = 0; c0 < n; c0 += U) {
+        float d[U], l[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u < n) {
+                d[u] = ws[(c0 + u) * size];
+                l[u] = less[c0 + u];
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c0 + u < n) {
+                ws[(c0 + u) * size] = S;
+                // as S + (less S + new): what a decay near 1 takes away keeps its own precision
+                S = l[u] == -1.0f ? d[u] : S + fmaf(l[u], S, d[u]);
+            }
+    }
+    if (p.a.state_out) p.a.state_out[at] = S;
+}
+
+template <class T>
+__global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams p) {
+    grid_begin();
+    extern __shared__ __align__(16) float smem[];
+    __shared__ Sums sums;
+    float *Q = smem, *K = Q + C * PITCH, *P = K + C * PITCH;        // K also holds tiles of V and of the state
+    const Place w = place_of(p);
+    if (!w.there) return;
+    const LinAttnParams &a = p.a;
+    T *out = (T *)a.out.p + token_base(a, a.out, w.b, w.s, w.h) + w.t0 * a.out.token;
+    if (w.s.slot < 0) {                     // not served: zeros
+        for (int i = 0; i < w.n; i++)
+            for (int c = threadIdx.x; c < a.dv; c += TPB) out[i * a.out.token + c] = from_f32<T>(0.0f);
+        return;
+    }
+    const T *q = (const T *)a.q.p + token_base(a, a.q, w.b, w.s, w.h / a.group) + w.t0 * a.q.token;
+    const T *k = (const T *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group) + w.t0 * a.k.token;
+    const T *v = (const T *)a.v.p + token_base(a, a.v, w.b, w.s, w.h) + w.t0 * a.v.token;
+    const float *S = p.ws + (size_t)blockIdx.x * a.dk * a.dv;
+    if (threadIdx.x < 32) sum_decays(p, a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr, w.n, sums);
+    const int row = threadIdx.x / 16 * 8, col = threadIdx.x % 16 * 4;
+    {
+        float f[8][4] = {};                 // keys row.. against queries col..
+        for (int d0 = 0; d0 < a.dk; d0 += C) {
+            __syncthreads();
+            load_tile<T, true>(Q, q, a.q.token, w.n, d0, a.dk);
+            load_tile<T, true>(K, k, a.k.token, w.n, d0, a.dk);
+            __syncthreads();
+            multiply(f, K, Q);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) P[(row + i) * PITCH + col + j] = col + j >= row + i ? f[i][j] * between(sums, col + j, row + i) : 0.0f;
+    }
+    for (int v0 = 0; v0 < a.dv; v0 += C) {
+        float f[8][4] = {};                 // queries row.., values col..
+        for (int d0 = 0; d0 < a.dk; d0 += C) {
+            __syncthreads();
+            if (a.dk > C) load_tile<T, true>(Q, q, a.q.token, w.n, d0, a.dk);
+            load_tile<float, false>(K, S + (size_t)d0 * a.dv, a.dv, min(C, a.dk - d0), v0, a.dv);
+            __syncthreads();
+            multiply(f, Q, K);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float e = sums.since[row + i] ? 0.0f : expf(sums.hi[row + i]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[i][j] *= e;
+        }
+        __syncthreads();
+        load_tile<T, false>(K, v, a.v.token, w.n, v0, a.dv);
+        __syncthreads();
+        multiply(f, P, K);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (row + i < w.n && v0 + col + j < a.dv) out[(row + i) * a.out.token + v0 + col + j] = from_f32<T>(a.scale * f[i][j]);
+    }
+}
+
+constexpr size_t tile_bytes(int n) { return (size_t)n * C * PITCH * sizeof(float); }
+
+template <class T>
+void launch(nb_handle_s *h, const SimtParams &p) {
+    auto out = linear_attention_output_kernel<T>;
+    const unsigned bit = sizeof(T) == 4 ? 16u : 32u;
+    if (!(h->linear_attention_ready & bit)) {
+        NB_CHECK_CUDA(cudaFuncSetAttribute(out, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tile_bytes(3)));
+        h->linear_attention_ready |= bit;
+    }
+    const dim3 grid((unsigned)(p.a.B * p.a.H * p.chunks));
+    launch_overlapped(h, linear_attention_contribution_kernel<T>, grid, TPB, tile_bytes(2), p);
+    check_launch("linear_attention_contribution_kernel");
+    const int blocks = (p.a.dk * p.a.dv + 255) / 256;
+    launch_overlapped(h, linear_attention_scan_kernel, dim3((unsigned)(p.a.B * p.a.H * blocks)), 256, 0, p, blocks);
+    check_launch("linear_attention_scan_kernel");
+    launch_overlapped(h, out, grid, TPB, tile_bytes(3), p);
+    check_launch("linear_attention_output_kernel");
+    count_launch(h, 3);
+}
+
+}  // namespace
+
+// In floats.  A state for every chunk: as much as the tensors themselves for heads of 64 values, twice that for 128.
+size_t linear_attention_simt_workspace(const nb_linear_attention_desc_t &d) {
+    const size_t chunks = (size_t)d.batch * d.heads * ((d.time_steps + C - 1) / C);
+    return chunks * ((size_t)d.key_dim * d.value_dim + 2);
+}
+void linear_attention_simt(nb_handle_s *h, const LinAttnParams &a, bool bf16, float *ws) {
+    SimtParams p = {};
+    p.a = a;
+    p.chunks = (a.T + C - 1) / C;
+    const size_t n = (size_t)a.B * a.H * p.chunks;
+    p.ws = ws;
+    p.less = ws + n * a.dk * a.dv;
+    p.odd = (int *)(p.less + n);
+    if (bf16) launch<__nv_bfloat16>(h, p);
+    else launch<float>(h, p);
+    linear_attention_repair(h, a, bf16, p.odd, p.chunks, p.ws);
+}
+
+}  // namespace nb
