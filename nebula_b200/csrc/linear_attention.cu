@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(STEP_TPB) linear_attention_step_kernel(LinAttn
 // shared memory; queries and keys are read from there as broadcasts.  Bound by the chain of tokens.
 constexpr int REC_TPB = 128, REC_TOK = 16, REC_COLS = 32;
 template <class T, int KR>
-__global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(LinAttnParams p, int tiles, const int *odd, int chunks, const float *ws) {
+__global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(LinAttnParams p, int tiles, const int *odd, int flags, int chunks, const float *ws) {
     grid_begin();
     __shared__ __align__(16) float qs[REC_TOK][4 * KR], ks[REC_TOK][4 * KR];
     __shared__ float vs[REC_TOK][REC_COLS], part[4][REC_TOK][REC_COLS], ds[REC_TOK];
@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(Lin
     if (odd) {                  // a repair
         int any = 0;
         if (s.slot >= 0)
-            for (int c = threadIdx.x; c * 64 < s.len; c += REC_TPB) any |= odd[bh * chunks + c];
+            for (int f = 0; f < flags; f++)
+                for (int c = threadIdx.x; c * 64 < s.len; c += REC_TPB) any |= odd[((long long)f * p.B * p.H + bh) * chunks + c];
         if (!__syncthreads_or(any)) return;
     }
     const T *q = (const T *)p.q.p + token_base(p, p.q, b, s, h / p.group), *k = (const T *)p.k.p + token_base(p, p.k, b, s, h / p.group);
@@ -181,10 +182,10 @@ __global__ void __launch_bounds__(REC_TPB) linear_attention_recurrent_kernel(Lin
 }
 
 template <class T>
-void launch_recurrent(nb_handle_s *h, const LinAttnParams &p, const int *odd = nullptr, int chunks = 0, const float *ws = nullptr) {
+void launch_recurrent(nb_handle_s *h, const LinAttnParams &p, const int *odd = nullptr, int flags = 0, int chunks = 0, const float *ws = nullptr) {
     const int tiles = (p.dv + REC_COLS - 1) / REC_COLS;
     const dim3 grid((unsigned)(p.B * p.H * tiles));
-    auto go = [&](auto kernel) { launch_overlapped(h, kernel, grid, REC_TPB, 0, p, tiles, odd, chunks, ws); };
+    auto go = [&](auto kernel) { launch_overlapped(h, kernel, grid, REC_TPB, 0, p, tiles, odd, flags, chunks, ws); };
     if (p.dk <= 16) go(linear_attention_recurrent_kernel<T, 4>);
     else if (p.dk <= 32) go(linear_attention_recurrent_kernel<T, 8>);
     else if (p.dk <= 64) go(linear_attention_recurrent_kernel<T, 16>);
@@ -216,9 +217,9 @@ void launch_step(nb_handle_s *h, const LinAttnParams &p) {
 
 }  // namespace
 
-void linear_attention_repair(nb_handle_s *h, const LinAttnParams &p, bool bf16, const int *odd, int chunks, const float *ws) {
-    if (bf16) launch_recurrent<__nv_bfloat16>(h, p, odd, chunks, ws);
-    else launch_recurrent<float>(h, p, odd, chunks, ws);
+void linear_attention_repair(nb_handle_s *h, const LinAttnParams &p, bool bf16, const int *odd, int flags, int chunks, const float *ws) {
+    if (bf16) launch_recurrent<__nv_bfloat16>(h, p, odd, flags, chunks, ws);
+    else launch_recurrent<float>(h, p, odd, flags, chunks, ws);
 }
 
 LinAttnPlan::LinAttnPlan(nb_handle_s *h, const nb_linear_attention_desc_t &desc) : nb_plan_s(NB_PLAN_LINEAR_ATTENTION, h), d(desc) {

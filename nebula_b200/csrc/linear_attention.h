@@ -68,10 +68,10 @@ size_t linear_attention_workspace(const nb_linear_attention_desc_t &d, const Lin
 void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAttnSplit &split, float *ws);
 
 // Prompts in chunks on the CUDA cores (linear_attention_simt.cu), and what it repairs with (linear_attention.cu): the recurrence for
-// the sequences and heads that have a chunk whose flag `odd` [B*H][chunks] is set, from the first of their states in `ws`.
+// the sequences and heads that have a chunk with one of its flags `odd` [flags][B*H][chunks] set, from the first of their states in `ws`.
 size_t linear_attention_simt_workspace(const nb_linear_attention_desc_t &d);
 void linear_attention_simt(nb_handle_s *h, const LinAttnParams &a, bool bf16, float *ws);
-void linear_attention_repair(nb_handle_s *h, const LinAttnParams &a, bool bf16, const int *odd, int chunks, const float *ws);
+void linear_attention_repair(nb_handle_s *h, const LinAttnParams &a, bool bf16, const int *odd, int flags, int chunks, const float *ws);
 
 struct LinAttnPlan : nb_plan_s {
     nb_linear_attention_desc_t d;

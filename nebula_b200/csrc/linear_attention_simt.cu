@@ -3,8 +3,9 @@
 //   1. each chunk's own contribution to the state, D_c = sum_j exp(G_end,j) k_j v_j^T, and its decay;
 //   2. the states in front of the chunks, S_{c+1} = exp(G_c) S_c + D_c, every value of a state by one thread;
 //   3. out_i = scale * [ sum_{j<=i} exp(G_ij) (q_i . k_j) v_j + exp(G_i) q_i^T S_c ].
-// Bound by fp32 arithmetic (C (dk + dv) + 2 dk dv FMAs a token and head); a thread has 8 x 4 values of a 64 x 64 product, so that
-// three 16-byte reads of shared memory feed 32 FMAs.
+// Bound by fp32 arithmetic (C (dk + dv) / 2 + 2 dk dv FMAs a token and head): a thread has 8 x 4 values of a 64 x 64 product, so that
+// three 16-byte reads of shared memory feed 32 FMAs, from tiles that lie as the tensors do (with transposed copies and 4-byte loads
+// 4 x 1023 tokens, 8 heads of 64 took 71 us, most of it waiting for loads).
 // G, the sums of log decays, are kept to 48 bits (two fp32 numbers), because the weight of two late tokens of a chunk is the
 // difference of two large sums.  A product with a masked weight of zero is NaN where v is not finite: the first launch looks for
 // such values, and the sequences and heads that have any are done once more, token by token.
@@ -25,7 +26,8 @@ struct SimtParams {
     int chunks;                 // of the longest sequence
     float *ws;                  // [B*H][chunks][dk][dv]: contributions, then the states in front of the chunks
     float *less;                // [B*H][chunks]: expm1 of a chunk's whole log decay, -1 where it holds a reset
-    int *odd;                   // [B*H][chunks]: the chunk's keys or values are not all finite
+    int *odd;                   // [tiles of a state][B*H][chunks]: the chunk's keys or values are not all finite
+    int vec[3], vec_state;      // q, k, v and the states: whole quads
 };
 
 // Sums of log decays from the chunk's start, resets left out, and the position of each token's last reset.
@@ -83,22 +85,55 @@ __device__ __forceinline__ Place place_of(const SimtParams &p) {
     return w;
 }
 
-// 64 x 64 values of a tensor, zeros where there are none: rows = tokens from `src` on, columns from `col` of `width`.
-// TRANSPOSED: [column][token].  Returns what is 0 if all are finite.
-template <class T, bool TRANSPOSED>
-__device__ __forceinline__ float load_tile(float *dst, const T *src, long long token, int n, int col, int width) {
+// 64 x 64 values of a tensor, zeros where there are none: rows = tokens from `src` on, columns from `col` of `width`, row r times by[r]
+// where there is such.  VEC: rows are whole quads on the boundaries of such.  Returns what is 0 if all are finite.
+template <class T> struct Quad;
+template <> struct Quad<float> { typedef float4 type; };
+template <> struct Quad<__nv_bfloat16> { typedef uint2 type; };
+__device__ __forceinline__ float4 quad_of(float4 v) { return v; }
+__device__ __forceinline__ float4 quad_of(uint2 v) {
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+template <class T>
+__device__ __forceinline__ float load_tile(float *dst, const T *src, long long token, int n, int col, int width, bool vec, const float *by = nullptr) {
+    const int c = threadIdx.x % 16 * 4, r0 = threadIdx.x / 16;
+    constexpr int N = C * 16 / TPB, STEP = TPB / 16;
+    const T *from = src + r0 * token + col + c;
+    float4 v[N];
+    if (vec) {
+        typename Quad<T>::type raw[N];
+#pragma unroll
+        for (int i = 0; i < N; i++, from += STEP * token) {
+            raw[i] = {};
+            if (r0 + i * STEP < n && col + c < width) raw[i] = *(const typename Quad<T>::type *)from;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = quad_of(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++, from += STEP * token) {
+            const int left = r0 + i * STEP < n ? width - col - c : 0;
+            v[i].x = left > 0 ? to_f32(from[0]) : 0.0f;
+            v[i].y = left > 1 ? to_f32(from[1]) : 0.0f;
+            v[i].z = left > 2 ? to_f32(from[2]) : 0.0f;
+            v[i].w = left > 3 ? to_f32(from[3]) : 0.0f;
+        }
+    }
     float seen = 0.0f;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < C * C; i += TPB) {
-        const int r = i / C, c = i % C;
-        const float v = r < n && col + c < width ? to_f32(src[r * token + col + c]) : 0.0f;
-        seen = fmaf(v, 0.0f, seen);
-        dst[TRANSPOSED ? c * PITCH + r : r * PITCH + c] = v;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int r = r0 + i * STEP;
+        seen = fmaf(v[i].x, 0.0f, fmaf(v[i].y, 0.0f, fmaf(v[i].z, 0.0f, fmaf(v[i].w, 0.0f, seen))));
+        if (by) {
+            const float w = by[r];
+            v[i].x *= w, v[i].y *= w, v[i].z *= w, v[i].w *= w;
+        }
+        *(float4 *)(dst + r * PITCH + c) = v[i];
     }
     return seen;
 }
 // f += A^T B for A [64 k][64 m], B [64 k][64 n] in shared memory; the thread's rows 8 (t / 16).., columns 4 (t % 16)..
-__device__ __forceinline__ void multiply(float (&f)[8][4], const float *A, const float *B) {
+__device__ __forceinline__ void multiply_tn(float (&f)[8][4], const float *A, const float *B) {
     const float *a = A + threadIdx.x / 16 * 8, *b = B + threadIdx.x % 16 * 4;
 #pragma unroll 8
     for (int k = 0; k < C; k++) {
@@ -110,12 +145,52 @@ __device__ __forceinline__ void multiply(float (&f)[8][4], const float *A, const
             for (int j = 0; j < 4; j++) f[i][j] = fmaf(u[i], v[j], f[i][j]);
     }
 }
+// f += A B for A [64 m][K k], B [K k][64 n]; the same rows and columns
+__device__ __forceinline__ void multiply_nn(float (&f)[8][4], const float *A, const float *B, int K) {
+    const float *a = A + threadIdx.x / 16 * 8 * PITCH, *b = B + threadIdx.x % 16 * 4;
+#pragma unroll 2
+    for (int k = 0; k < K; k += 4) {
+        float4 u[8], v[4];
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = *(const float4 *)(a + i * PITCH + k);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = *(const float4 *)(b + (k + e) * PITCH);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x = (&u[i].x)[e];
+                f[i][0] = fmaf(x, v[e].x, f[i][0]);
+                f[i][1] = fmaf(x, v[e].y, f[i][1]);
+                f[i][2] = fmaf(x, v[e].z, f[i][2]);
+                f[i][3] = fmaf(x, v[e].w, f[i][3]);
+            }
+    }
+}
+// f += A B^T for A [64 m][64 k], B [64 n][64 k]; the thread's rows 8 (t / 16).., columns t % 16 + 16 j, for j up to `last`
+__device__ __forceinline__ void multiply_nt(float (&f)[8][4], const float *A, const float *B, int last) {
+    const float *a = A + threadIdx.x / 16 * 8 * PITCH, *b = B + threadIdx.x % 16 * PITCH;
+#pragma unroll 2
+    for (int k = 0; k < C; k += 4) {
+        float4 u[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = *(const float4 *)(a + i * PITCH + k);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > last) break;
+            const float4 v = *(const float4 *)(b + j * 16 * PITCH + k);
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i][j] = fmaf(u[i].x, v.x, fmaf(u[i].y, v.y, fmaf(u[i].z, v.z, fmaf(u[i].w, v.w, f[i][j]))));
+        }
+    }
+}
 
 template <class T>
 __global__ void __launch_bounds__(TPB) linear_attention_contribution_kernel(SimtParams p) {
     grid_begin();
     extern __shared__ __align__(16) float smem[];
     __shared__ Sums sums;
+    __shared__ float by[C];
     float *K = smem, *V = smem + C * PITCH;
     const Place w = place_of(p);
     if (!w.there || w.s.slot < 0) return;
@@ -123,35 +198,34 @@ __global__ void __launch_bounds__(TPB) linear_attention_contribution_kernel(Simt
     const T *k = (const T *)a.k.p + token_base(a, a.k, w.b, w.s, w.h / a.group) + w.t0 * a.k.token;
     const T *v = (const T *)a.v.p + token_base(a, a.v, w.b, w.s, w.h) + w.t0 * a.v.token;
     if (threadIdx.x < 32) sum_decays(p, a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr, w.n, sums);
+    // a tile of the state: y = its number
+    const int d0 = blockIdx.y % ((a.dk + C - 1) / C) * C, v0 = blockIdx.y / ((a.dk + C - 1) / C) * C;
+    float seen = load_tile<T>(V, v, a.v.token, w.n, v0, a.dv, p.vec[2]);
+    __syncthreads();
+    if (threadIdx.x < C) by[threadIdx.x] = between(sums, C - 1, threadIdx.x);
+    __syncthreads();
+    seen += load_tile<T>(K, k, a.k.token, w.n, d0, a.dk, p.vec[1], by);       // the weights go to the keys
+    const int odd = __syncthreads_or(!(seen == 0.0f));
+    float f[8][4] = {};
+    multiply_tn(f, K, V);
     float *D = p.ws + (size_t)blockIdx.x * a.dk * a.dv;
-    float seen = 0.0f;
-    for (int d0 = 0; d0 < a.dk; d0 += C) {
-        __syncthreads();
-        seen += load_tile<T, false>(K, k, a.k.token, w.n, d0, a.dk);
-        __syncthreads();
-        if (threadIdx.x < C) {                          // the weights go to the keys
-            const float by = between(sums, C - 1, threadIdx.x);
-            for (int c = 0; c < C; c++) K[threadIdx.x * PITCH + c] *= by;
-        }
-        for (int v0 = 0; v0 < a.dv; v0 += C) {
-            __syncthreads();
-            seen += load_tile<T, false>(V, v, a.v.token, w.n, v0, a.dv);
-            __syncthreads();
-            float f[8][4] = {};
-            multiply(f, K, V);
+    const int c = v0 + threadIdx.x % 16 * 4;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+    for (int i = 0; i < 8; i++) {
+        const int r = d0 + threadIdx.x / 16 * 8 + i;
+        if (r >= a.dk) continue;
+        float *to = D + (size_t)r * a.dv + c;
+        if (p.vec_state) {
+            if (c < a.dv) *(float4 *)to = make_float4(f[i][0], f[i][1], f[i][2], f[i][3]);
+        } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int r = d0 + threadIdx.x / 16 * 8 + i, c = v0 + threadIdx.x % 16 * 4 + j;
-                    if (r < a.dk && c < a.dv) D[(size_t)r * a.dv + c] = f[i][j];
-                }
+            for (int j = 0; j < 4; j++)
+                if (c + j < a.dv) to[j] = f[i][j];
         }
     }
-    const int odd = __syncthreads_or(!(seen == 0.0f));
     if (threadIdx.x == 0) {
-        p.odd[blockIdx.x] = odd;
-        p.less[blockIdx.x] = sums.since[C - 1] ? -1.0f : expm1f(sums.total);
+        p.odd[blockIdx.y * gridDim.x + blockIdx.x] = odd;
+        if (blockIdx.y == 0) p.less[blockIdx.x] = sums.since[C - 1] ? -1.0f : expm1f(sums.total);
     }
 }
 
@@ -207,29 +281,33 @@ __global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams
     const T *v = (const T *)a.v.p + token_base(a, a.v, w.b, w.s, w.h) + w.t0 * a.v.token;
     const float *S = p.ws + (size_t)blockIdx.x * a.dk * a.dv;
     if (threadIdx.x < 32) sum_decays(p, a.g.p ? (const float *)a.g.p + token_base(a, a.g, w.b, w.s, w.h) + w.t0 * a.g.token : nullptr, w.n, sums);
-    const int row = threadIdx.x / 16 * 8, col = threadIdx.x % 16 * 4;
+    const int row = threadIdx.x / 16 * 8, block = threadIdx.x / 32;     // the thread's queries, in which block of 16
     {
-        float f[8][4] = {};                 // keys row.. against queries col..
+        float f[8][4] = {};                 // queries row.. against keys t % 16 + 16 j, which lie in block j
         for (int d0 = 0; d0 < a.dk; d0 += C) {
+            if (d0) __syncthreads();
+            load_tile<T>(Q, q, a.q.token, w.n, d0, a.dk, p.vec[0]);
+            load_tile<T>(K, k, a.k.token, w.n, d0, a.dk, p.vec[1]);
             __syncthreads();
-            load_tile<T, true>(Q, q, a.q.token, w.n, d0, a.dk);
-            load_tile<T, true>(K, k, a.k.token, w.n, d0, a.dk);
-            __syncthreads();
-            multiply(f, K, Q);
+            multiply_nt(f, Q, K, block);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) P[(row + i) * PITCH + col + j] = col + j >= row + i ? f[i][j] * between(sums, col + j, row + i) : 0.0f;
+            for (int j = 0; j < 4; j++) {
+                const int key = threadIdx.x % 16 + 16 * j;
+                if (j <= block) P[(row + i) * PITCH + key] = row + i >= key ? f[i][j] * between(sums, row + i, key) : 0.0f;
+            }
     }
+    const int col = threadIdx.x % 16 * 4;
     for (int v0 = 0; v0 < a.dv; v0 += C) {
         float f[8][4] = {};                 // queries row.., values col..
         for (int d0 = 0; d0 < a.dk; d0 += C) {
             __syncthreads();
-            if (a.dk > C) load_tile<T, true>(Q, q, a.q.token, w.n, d0, a.dk);
-            load_tile<float, false>(K, S + (size_t)d0 * a.dv, a.dv, min(C, a.dk - d0), v0, a.dv);
+            if (a.dk > C) load_tile<T>(Q, q, a.q.token, w.n, d0, a.dk, p.vec[0]);
+            load_tile<float>(K, S + (size_t)d0 * a.dv, a.dv, min(C, a.dk - d0), v0, a.dv, p.vec_state);
             __syncthreads();
-            multiply(f, Q, K);
+            multiply_nn(f, Q, K, C);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -238,9 +316,9 @@ __global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams
             for (int j = 0; j < 4; j++) f[i][j] *= e;
         }
         __syncthreads();
-        load_tile<T, false>(K, v, a.v.token, w.n, v0, a.dv);
+        load_tile<T>(K, v, a.v.token, w.n, v0, a.dv, p.vec[2]);
         __syncthreads();
-        multiply(f, P, K);
+        multiply_nn(f, P, K, 16 * (block + 1));         // keys of later blocks are not seen
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -249,6 +327,7 @@ __global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams
     }
 }
 
+int state_tiles(int dk, int dv) { return ((dk + C - 1) / C) * ((dv + C - 1) / C); }
 constexpr size_t tile_bytes(int n) { return (size_t)n * C * PITCH * sizeof(float); }
 
 template <class T>
@@ -260,7 +339,7 @@ void launch(nb_handle_s *h, const SimtParams &p) {
         h->linear_attention_ready |= bit;
     }
     const dim3 grid((unsigned)(p.a.B * p.a.H * p.chunks));
-    launch_overlapped(h, linear_attention_contribution_kernel<T>, grid, TPB, tile_bytes(2), p);
+    launch_overlapped(h, linear_attention_contribution_kernel<T>, dim3(grid.x, (unsigned)state_tiles(p.a.dk, p.a.dv)), TPB, tile_bytes(2), p);
     check_launch("linear_attention_contribution_kernel");
     const int blocks = (p.a.dk * p.a.dv + 255) / 256;
     launch_overlapped(h, linear_attention_scan_kernel, dim3((unsigned)(p.a.B * p.a.H * blocks)), 256, 0, p, blocks);
@@ -275,7 +354,7 @@ void launch(nb_handle_s *h, const SimtParams &p) {
 // In floats.  A state for every chunk: as much as the tensors themselves for heads of 64 values, twice that for 128.
 size_t linear_attention_simt_workspace(const nb_linear_attention_desc_t &d) {
     const size_t chunks = (size_t)d.batch * d.heads * ((d.time_steps + C - 1) / C);
-    return chunks * ((size_t)d.key_dim * d.value_dim + 2);
+    return chunks * ((size_t)d.key_dim * d.value_dim + 1 + state_tiles(d.key_dim, d.value_dim));
 }
 void linear_attention_simt(nb_handle_s *h, const LinAttnParams &a, bool bf16, float *ws) {
     SimtParams p = {};
@@ -283,11 +362,19 @@ void linear_attention_simt(nb_handle_s *h, const LinAttnParams &a, bool bf16, fl
     p.chunks = (a.T + C - 1) / C;
     const size_t n = (size_t)a.B * a.H * p.chunks;
     p.ws = ws;
-    p.less = ws + n * a.dk * a.dv;
+    p.less = ws + n * a.dk * a.dv;      // (behind the states)
     p.odd = (int *)(p.less + n);
+    const int quad = bf16 ? 8 : 16;
+    auto whole = [&](const TokenView &t, int dim) {
+        return (uintptr_t)t.p % quad == 0 && ((a.offsets ? 0 : t.batch) | t.token | t.head) % 4 == 0 && dim % 4 == 0;
+    };
+    p.vec[0] = whole(a.q, a.dk);
+    p.vec[1] = whole(a.k, a.dk);
+    p.vec[2] = whole(a.v, a.dv);
+    p.vec_state = a.dv % 4 == 0;        // (the states lie one behind the other from an aligned start)
     if (bf16) launch<__nv_bfloat16>(h, p);
     else launch<float>(h, p);
-    linear_attention_repair(h, a, bf16, p.odd, p.chunks, p.ws);
+    linear_attention_repair(h, a, bf16, p.odd, state_tiles(a.dk, a.dv), p.chunks, p.ws);
 }
 
 }  // namespace nb
