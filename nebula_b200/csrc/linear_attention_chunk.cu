@@ -3,12 +3,12 @@
 // With positions i, j of a chunk, G_ij the sum of the log decays of tokens j+1 .. i, and S the state before the chunk:
 //   out_i = scale * [ sum_{j<=i} exp(G_ij) (q_i . k_j) v_j  +  exp(G_i) q_i^T S ],   G_i from the chunk's start
 //   S'    = exp(G_end) S + sum_j exp(G_end,j) k_j v_j^T
-// Everything is computed transposed, with the 128 accumulator lanes being the values of a head (or the keys j), because then both
-// products that weights have to be put into first take them from tensor memory, and the state keeps one lane's row in one thread:
+// Everything is computed transposed, with the 128 accumulator lanes being the values of a head (or the keys j), because then the
+// weighted values go to tensor memory, and the state keeps one lane's row in one thread:
 //   A^T [j][i]    = K Q^T                M = 64, N = 64
 //   O1^T [dv][i]  = V^T P^T              P = A masked and weighted, bf16, in shared memory
-//   O2^T [dv][i]  = S^T Q^T              S rounded to bf16, in tensor memory
-//   D^T [dv][dk]  = (V w)^T K            w_j = exp(G_end,j); V w in three bf16 terms, in tensor memory
+//   O2^T [dv][i]  = S^T Q^T              S rounded to bf16, in shared memory
+//   D^T [dv][dk]  = (V w)^T K            w_j = exp(G_end,j); V w in three bf16 terms, in tensor memory, for two chunks in turn
 // The state itself is fp32, in the registers of eight warps, and so are all exponents.  What is rounded to bf16: P and the S that
 // the queries read (each a relative 2^-9 of a term of a sum whose result is rounded to bf16 anyway).  V w is not rounded: a
 // product of 24 bits is cut into three terms of 8, exactly, since the state is an fp32 result that lives on.
@@ -49,7 +49,7 @@ constexpr int SLOTS = 8;                    // of the decays' ring: more than th
 constexpr int MAX_STAGES = 5;
 constexpr float RESET = -104.0f;            // exp of this and less is 0 in fp32
 // columns of tensor memory
-constexpr uint32_t T_KQ = 0, T_O2 = 64, T_O1 = 128, T_D = 192, T_S = 320, T_VW = 384, T_COLS = 512;
+constexpr uint32_t T_KQ = 0, T_O2 = 64, T_O1 = 128, T_D = 192, T_VW = 320, T_VW_STEP = 96, T_COLS = 512;
 
 // What the log decays of a chunk come to.
 struct Decays {
@@ -62,9 +62,9 @@ struct Decays {
 };
 
 struct ChunkParams {
-    CUtensorMap maps[3];                // q, k, v: {values, heads, tokens, sequences}, boxes of 64 values x 64 tokens; where tma
+    CUtensorMap maps[4];                // q, k, v, out: {values, heads, tokens, sequences}, boxes of 64 values x 64 tokens; where tma
     LinAttnParams a;
-    int tma;                            // whole chunks come by TMA
+    int tma, tma_out;                   // whole chunks come, and go, by TMA
     int splits, chunks_per_split;       // of the axis of tokens
     float *ws;                          // [B*H][splits - 1][dk][dv]: states at the splits
     float *ws_less;                     // [B*H][splits - 1]: expm1 of each split's log decay
@@ -115,13 +115,6 @@ __device__ __forceinline__ void umma_done(uint32_t leader, uint64_t *bar) {
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t mn_step) {
     return ((uint64_t)SMEM_DESC_HI << 32) | ((addr >> 4) & 0x3FFF) | ((mn_step >> 4) << 16);
 }
-__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t *v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]),
-        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
-        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
-        : "memory");
-}
 // (The roles' warps run converged: every wait ends with that.)
 __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
@@ -135,7 +128,21 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&v)[32]) 
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// All loads so far have arrived.  Takes the registers that are read next, so that nothing that reads them moves in front of it.
+__device__ __forceinline__ void tmem_loads_done(uint32_t (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])::"memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_loads_done(uint32_t (&v)[N], uint32_t (&w)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]), "+r"(w[i]));
+}
+__device__ __forceinline__ void tmem_loads_done(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(v[i]));
+}
 __device__ __forceinline__ void tmem_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 16 lanes of tensor memory in the layout of matrix fragments: thread t holds rows t / 4 and t / 4 + 8.  Loads: of every eight columns
 // 2 (t % 4) and the next one, of both rows; stores of four columns: column t % 4, of both rows.
@@ -305,12 +312,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023);     // (an offset, so that accesses stay those of shared memory)
     const int stages = p.stages;
     uint8_t *P = smem + stages * STAGE;                 // [2][64 keys][64 queries] bf16, swizzled like the tiles
-    __nv_bfloat16 *O = (__nv_bfloat16 *)(P + 2 * HALF_TILE);        // [64 queries][128], groups of eight values at (group ^ query % 8)
-    Decays *dec = (Decays *)((uint8_t *)O + C * 128 * 2);
+    __nv_bfloat16 *O = (__nv_bfloat16 *)(P + 2 * HALF_TILE);        // [2][64 queries][64 values], swizzled like the tiles
+    uint8_t *ST = (uint8_t *)O + 2 * HALF_TILE;           // [KH][128 values][64 keys] bf16, swizzled like the tiles
+    Decays *dec = (Decays *)(ST + KH * 2 * HALF_TILE);
     uint64_t *bars = (uint64_t *)(dec + SLOTS);
     uint64_t *full = bars, *empty = bars + MAX_STAGES;  // loaders -> all, MMA -> loaders
     uint64_t *kq_full = empty + MAX_STAGES, *kq_empty = kq_full + 1, *p_full = kq_empty + 1 /* [2] */, *o_full = p_full + 2, *o_empty = o_full + 1;
-    uint64_t *v_full = o_empty + 1, *d_empty = v_full + 1, *d_full = d_empty + 1, *s_full = d_full + 1, *s_empty = s_full + 1;
+    uint64_t *v_full = o_empty + 1 /* [2] */, *v_empty = v_full + 2 /* [2] */, *d_empty = v_empty + 2, *d_full = d_empty + 1, *s_full = d_full + 1, *s_empty = s_full + 1;
     uint32_t *tmem_slot = (uint32_t *)(s_empty + 1);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     int *odd = (int *)(tmem_slot + 2);                  // infinities or NaN were met
@@ -328,7 +336,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         mbar_init(&p_full[1], PAIR_WARPS);
         mbar_init(o_full, 1);
         mbar_init(o_empty, OUT_WARPS);
-        mbar_init(v_full, TERM_WARPS);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&v_full[i], TERM_WARPS);
+            mbar_init(&v_empty[i], 1);
+        }
         mbar_init(d_empty, STATE_WARPS);
         mbar_init(d_full, 1);
         mbar_init(s_full, STATE_WARPS);
@@ -382,16 +393,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
         for (int n = 0; n < N; n++) {
             if (!STATES_ONLY) {                         // what the queries read
                 wait(s_empty, (n - 1) & 1);             // (at first: at once)
-                tc_fence_after();
+                uint8_t *row = ST + (half * R / 64) * 2 * HALF_TILE + dv * 128;
 #pragma unroll
-                for (int c = 0; c < R / 2; c += 16) {
-                    uint32_t x[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) x[i] = pack_bf16(S[c + i].x, S[c + i].y);
-                    tmem_st_32x16(at + T_S + half * (R / 2) + c, x);
-                }
-                tmem_stores_done();
-                tc_fence_before();
+                for (int c = 0; c < R / 8; c++)
+                    *(uint4 *)(row + (((half * R / 8 + c & 7) ^ (dv & 7)) << 4)) =
+                        make_uint4(pack_bf16(S[4 * c].x, S[4 * c].y), pack_bf16(S[4 * c + 1].x, S[4 * c + 1].y), pack_bf16(S[4 * c + 2].x, S[4 * c + 2].y),
+                                   pack_bf16(S[4 * c + 3].x, S[4 * c + 3].y));
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_full);
             }
@@ -402,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
             for (int c = 0; c < R; c += 32) {
                 uint32_t d[32];
                 tmem_load_32(at + T_D + half * R + c, d);
-                tmem_loads_done();
+                tmem_loads_done(d);
                 // as S + (less S + new): what a decay near 1 takes away keeps its own precision.  Once a value is not finite it
                 // stays so, whatever the decays
 #pragma unroll
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     float2 x[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) x[i] = mul2(make_float2(low_value(v[i]), high_value(v[i])), by[i / 2]);
-                    if (h == 0) wait(d_full, (n - 1) & 1);          // the terms in tensor memory have been read (at first: at once)
+                    if (h == 0) wait(&v_empty[n & 1], (n >> 1) - 1 & 1);        // the terms of two chunks before have been read (at first: at once)
                     tc_fence_after();
 #pragma unroll
                     for (int term = 0; term < 3; term++) {
@@ -467,16 +475,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                             y[i] = pack_high(x[i].x, x[i].y);
                             if (term < 2) x[i] = fma2(make_float2(-1.0f, -1.0f), make_float2(high_part(x[i].x), high_part(x[i].y)), x[i]);
                         }
-                        tmem_st_16x128_x4(at + ((uint32_t)(h * 16) << 16) + term * 32, y);
+                        tmem_st_16x128_x4(at + ((uint32_t)(h * 16) << 16) + (n & 1) * T_VW_STEP + term * 32, y);
                     }
                 }
                 tmem_stores_done();
             } else {
-                wait(d_full, (n - 1) & 1);
+                wait(&v_empty[n & 1], (n >> 1) - 1 & 1);
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full);
+            if (lane == 0) mbar_arrive(&v_full[n & 1]);
             if (++stage == stages) stage = 0, phase ^= 1;
         }
         tc_fence_before();
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     tmem_ld_16x256_x2(at + g * 8, x);
                     const float2 s = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + i1), t = *(const float2 *)(d.sum2 + quarter * 16 + g * 8 + 8 + i1);
                     const float e[8] = {ex2(s.x + m0), ex2(s.y + m0), ex2(s.x + m1), ex2(s.y + m1), ex2(t.x + m0), ex2(t.y + m0), ex2(t.x + m1), ex2(t.y + m1)};
-                    tmem_loads_done();
+                    tmem_loads_done(x);
                     uint32_t y[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) y[i] = pack_bf16(__uint_as_float(x[2 * i]) * e[2 * i], __uint_as_float(x[2 * i + 1]) * e[2 * i + 1]);
@@ -619,19 +627,20 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
 #pragma unroll 1
             for (int n = 0; n < N; n++) {
                 wait(o_full, n & 1);
+                if (t == 0) tma_store_wait_read<0>();
                 epilogue_bar_sync(1);                       // the outputs of the chunk before have left shared memory
                 tc_fence_after();
                 if (quarter * 32 < a.dv) {
                     const float *weight = dec[n % SLOTS].from_start + 2 * (lane & 3);
 #pragma unroll 1
                     for (int h = 0; h < 4; h++) {       // 16 values of the head, 32 tokens
-                        const uint32_t to = smem_u32(O) + ((h & 1) * 32 + (lane >> 4) * 8 + (lane & 7)) * 256 +
-                                            (((quarter * 4 + (h & 2) + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
+                        const uint32_t to = smem_u32(O) + (quarter >> 1) * HALF_TILE + ((h & 1) * 32 + (lane >> 4) * 8 + (lane & 7)) * 128 +
+                                            ((((quarter & 1) * 4 + (h & 2) + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
                         const uint32_t from = at + ((uint32_t)((h & 2) * 8) << 16) + (h & 1) * 32;
                         uint32_t x[16], y[16];
                         tmem_ld_16x256_x4(from + T_O2, x);
                         tmem_ld_16x256_x4(from + T_O1, y);
-                        tmem_loads_done();
+                        tmem_loads_done(x, y);
 #pragma unroll
                         for (int g = 0; g < 4; g++) {
                             const float2 e = *(const float2 *)(weight + (h & 1) * 32 + g * 8);
@@ -639,33 +648,36 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                             const float2 o1 = fma2(e, as_float2(x[4 * g + 2], x[4 * g + 3]), as_float2(y[4 * g + 2], y[4 * g + 3]));
                             x[4 * g] = pack_bf16(o0.x, o0.y);
                             x[4 * g + 1] = pack_bf16(o1.x, o1.y);
-                            if (g & 1) stmatrix_trans(to + (g - 1) * 8 * 256, x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
+                            if (g & 1) stmatrix_trans(to + (g - 1) * 8 * 128, x[4 * g - 4], x[4 * g - 3], x[4 * g], x[4 * g + 1]);
                         }
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_empty);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 epilogue_bar_sync(1);
                 const int t0 = w.t0 + n * C, m = min(C, w.n - n * C);
-                if (p.out_vec) {
-                    const int c = t & 15;
-                    if (c * 8 < a.dv) {
-                        const __nv_bfloat16 *from = O + (t >> 4) * 128 + ((c ^ (t >> 4)) << 3);
-                        __nv_bfloat16 *to = out + (t0 + (t >> 4)) * a.out.token + c * 8;
-                        if (m == C) {
-#pragma unroll 4
-                            for (int i = 0; i < 8; i++, to += 8 * a.out.token) *(uint4 *)to = *(const uint4 *)(from + i * 8 * 128);
-                        } else {
-#pragma unroll 1
-                            for (int i = t >> 4; i < m; i += 8, to += 8 * a.out.token, from += 8 * 128) *(uint4 *)to = *(const uint4 *)from;
-                        }
+                if (p.tma_out && m == C) {
+                    if (t == 0) {
+                        const int token = a.offsets ? (int)w.s.first + t0 : t0, sequence = a.offsets ? 0 : w.b;
+                        for (int i = 0; i * 64 < a.dv; i++) tma_store_4d(&p.maps[3], (uint8_t *)O + i * HALF_TILE, i * 64, w.h, token, sequence);
+                        tma_store_commit();
                     }
+                } else if (p.out_vec) {
+                    const int c = t & 15;
+                    if (c * 8 < a.dv)
+#pragma unroll 1
+                        for (int i = t >> 4; i < m; i += 8)
+                            *(uint4 *)(out + (t0 + i) * a.out.token + c * 8) = *(const uint4 *)((uint8_t *)O + (c >> 3) * HALF_TILE + i * 128 + ((c & 7 ^ i & 7) << 4));
                 } else if (t < a.dv) {
 #pragma unroll 1
-                    for (int i = 0; i < m; i++) out[(t0 + i) * a.out.token + t] = O[i * 128 + (((t >> 3) ^ (i & 7)) << 3) + (t & 7)];
+                    for (int i = 0; i < m; i++)
+                        out[(t0 + i) * a.out.token + t] =
+                            *(const __nv_bfloat16 *)((uint8_t *)O + (t >> 6) * HALF_TILE + i * 128 + (((t >> 3 & 7) ^ i & 7) << 4) + (t & 7) * 2);
                 }
             }
+            if (t == 0) tma_store_wait_all();
         }
         tc_fence_before();
         __syncthreads();
@@ -792,15 +804,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     const uint32_t k = smem_u32(smem) + stage * STAGE;
                     tiles();
                     wait(d_empty, (n - 1) & 1);
-                    wait(v_full, n & 1);
+                    wait(&v_full[n & 1], n >> 1 & 1);
                     tc_fence_after();
 #pragma unroll 1
                     for (int term = 2; term >= 0; term--)
 #pragma unroll
                         for (int i = 0; i < C / 16; i++)
-                            umma_bf16_ts(leader, tmem + T_D, tmem + T_VW + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
+                            umma_bf16_ts(leader, tmem + T_D, tmem + T_VW + (n & 1) * T_VW_STEP + term * 32 + i * 8, tile_desc(k + i * 2048, HALF_TILE),
                                          idesc_bf16(128, DK, 0, 1), term != 2 || i != 0);
                     umma_done(leader, d_full);
+                    umma_done(leader, &v_empty[n & 1]);
                     umma_done(leader, &empty[stage]);
                     if (++stage == stages) stage = 0;
                 }
@@ -829,8 +842,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
                     for (int h = 0; h < KH; h++)
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            umma_bf16_ts(leader, tmem + T_O2, tmem + T_S + h * 32 + i * 8, tile_desc(q + h * HALF_TILE + i * 32, 16),
-                                         idesc_bf16(128, C, 0, 0), (h | i) != 0);
+                            umma_bf16(leader, tmem + T_O2, tile_desc(smem_u32(ST) + h * 2 * HALF_TILE + i * 32, 16), tile_desc(q + h * HALF_TILE + i * 32, 16),
+                                      idesc_bf16(128, C, 0, 0), (h | i) != 0);
                     umma_done(leader, s_empty);
                     wait(&p_full[n & 1], n >> 1 & 1);
                     const uint32_t pt = smem_u32(P) + (n & 1) * HALF_TILE;
@@ -887,7 +900,7 @@ constexpr int stage_bytes() { return (2 * (DK / 64) + 2) * HALF_TILE; }
 template <int DK>
 constexpr int stages_of() { return DK == 128 ? 3 : MAX_STAGES; }
 template <int DK>
-constexpr size_t smem_bytes() { return 1024 + stages_of<DK>() * stage_bytes<DK>() + 2 * HALF_TILE + C * 128 * 2 + SLOTS * sizeof(Decays) + 256; }
+constexpr size_t smem_bytes() { return 1024 + stages_of<DK>() * stage_bytes<DK>() + 2 * HALF_TILE + 2 * HALF_TILE + DK / 64 * 2 * HALF_TILE + SLOTS * sizeof(Decays) + 256; }
 
 template <int DK, bool STATES_ONLY>
 void launch_chunks(nb_handle_s *h, const ChunkParams &p) {
@@ -909,14 +922,14 @@ void launch_chunks(nb_handle_s *h, const ChunkParams &p) {
 }
 
 // The tensor map of a tensor of tokens.  False where it cannot have one: strides that repeat values, or the columns that its boxes
-// have past a row's last value (which arrive as zeros, but are read) not surely inside the tensor's allocation.
-bool map_tokens(nb_handle_s *h, const LinAttnParams &a, const TokenView &t, int heads, int dim, CUtensorMap *map) {
+// have past a row's last value (which arrive as zeros, but are read; stores leave them out) not surely inside the tensor's allocation.
+bool map_tokens(nb_handle_s *h, const LinAttnParams &a, const TokenView &t, int heads, int dim, CUtensorMap *map, bool read = true) {
     const long long tokens = a.offsets ? a.tokens : a.T, sequences = a.offsets ? 1 : a.B;
     if (tokens < C) return false;
     if ((heads > 1 && t.head == 0) || t.token == 0 || (sequences > 1 && t.batch == 0)) return false;
     const int box = (dim + 63) / 64 * 64;
     const long long last = (sequences - 1) * t.batch + (tokens - 1) * t.token + (heads - 1) * t.head;
-    if (box != dim && !extent_inside(h, t.p, (last + box) * 2)) return false;
+    if (read && box != dim && !extent_inside(h, t.p, (last + box) * 2)) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)sequences};
     const cuuint64_t strides[3] = {(cuuint64_t)(heads > 1 ? t.head * 2 : 16), (cuuint64_t)t.token * 2, (cuuint64_t)(sequences > 1 ? t.batch * 2 : 16)};
     for (cuuint64_t s : strides)
@@ -978,6 +991,7 @@ void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAt
     p.out_vec = whole(a.out, a.dv, false);
     p.tma = p.vec[0] && p.vec[1] && p.vec[2] && map_tokens(h, a, a.q, a.H / a.group, a.dk, &p.maps[0]) &&
             map_tokens(h, a, a.k, a.H / a.group, a.dk, &p.maps[1]) && map_tokens(h, a, a.v, a.H, a.dv, &p.maps[2]);
+    p.tma_out = p.out_vec && map_tokens(h, a, a.out, a.H, a.dv, &p.maps[3], false);
     const bool wide = a.dk > 64;
     p.stages = wide ? stages_of<128>() : stages_of<64>();
     if (p.splits > 1) {
