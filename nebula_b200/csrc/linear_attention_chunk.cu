@@ -47,6 +47,7 @@ static_assert(THREADS == 896 && 2 * STATE_REGS + 2 * TERM_REGS + PAIR_REGS + OUT
 constexpr int HALF_TILE = C * 128;          // [64 tokens][64 values] of bf16, rows of 128 bytes, 128-byte swizzle
 constexpr int SLOTS = 8;                    // of the decays' ring: more than the stages of the tiles' plus two chunks
 constexpr int MAX_STAGES = 5;
+constexpr int MAX_ORDERED = 512;            // sequences that are put in the order of their lengths
 constexpr float RESET = -104.0f;            // exp of this and less is 0 in fp32
 // columns of tensor memory
 constexpr uint32_t T_KQ = 0, T_O2 = 64, T_O1 = 128, T_D = 192, T_VW = 320, T_VW_STEP = 96, T_COLS = 512;
@@ -72,6 +73,7 @@ struct ChunkParams {
     int out_vec;
     float scale, log2_size;             // and the logarithm of its size
     unsigned negative;                  // scale < 0
+    int longest_first;                  // CTAs take the sequences in the order of their lengths
     int stages;
     int *status;
 };
@@ -249,12 +251,12 @@ struct Work {
     int split;
 };
 template <bool STATES_ONLY>
-__device__ __forceinline__ Work work_of(const ChunkParams &p) {
+__device__ __forceinline__ Work work_of(const ChunkParams &p, int sequence) {
     Work w;
     const int split = blockIdx.x % (STATES_ONLY ? p.splits - 1 : p.splits), bh = blockIdx.x / (STATES_ONLY ? p.splits - 1 : p.splits);
     const long long size = (long long)p.a.dk * p.a.dv;
     w.h = bh % p.a.H;
-    w.b = bh / p.a.H;
+    w.b = sequence >= 0 ? sequence : bh / p.a.H;
     w.s = seq_at(p.a, w.b);
     w.split = split;
     const int span = p.chunks_per_split * C;
@@ -322,6 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     uint32_t *tmem_slot = (uint32_t *)(s_empty + 1);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     int *odd = (int *)(tmem_slot + 2);                  // infinities or NaN were met
+    int *sequence = (int *)(tmem_slot + 3);             // the CTA's, where they do not go by their numbers
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_dependents_start();
@@ -366,7 +369,18 @@ __global__ void __launch_bounds__(THREADS, 1) linear_attention_chunk_kernel(cons
     grid_dependency_wait();
 
     const LinAttnParams &a = p.a;
-    const Work w = work_of<STATES_ONLY>(p);
+    if (!STATES_ONLY && p.longest_first) {          // CTAs start in the order of their numbers
+        int *lens = (int *)dec;
+        if (tid < a.B) lens[tid] = seq_at(a, tid).len;
+        __syncthreads();
+        if (tid < a.B) {
+            int before = 0;
+            for (int i = 0; i < a.B; i++) before += lens[i] > lens[tid] || (lens[i] == lens[tid] && i < tid);
+            if (before == (int)(blockIdx.x / a.H)) *sequence = tid;
+        }
+        __syncthreads();
+    }
+    const Work w = work_of<STATES_ONLY>(p, !STATES_ONLY && p.longest_first ? *sequence : -1);
     const bool served = w.s.slot >= 0 && !w.skip;
     const int N = served ? (w.n + C - 1) / C : 0;
     const Waits wait = {abort_flag, p.status};
@@ -888,10 +902,21 @@ __global__ void __launch_bounds__(256) linear_attention_join_kernel(const __grid
     float S = p.a.state ? p.a.state[(s.slot * p.a.H + h) * size + i] : 0.0f;
     float *ws = p.ws + (long long)bh * (p.splits - 1) * size + i;
     const float *less = p.ws_less + (long long)bh * (p.splits - 1);
-    for (int k = 0; k < n; k++) {
-        const float own = ws[k * size], l = less[k];
-        S = l == -1.0f ? own : S + fmaf(l, S, own);
-        ws[k * size] = S;
+    constexpr int U = 8;                // states asked for at once
+    for (int k0 = 0; k0 < n; k0 += U) {
+        float own[U], l[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (k0 + u < n) {
+                own[u] = ws[(k0 + u) * size];
+                l[u] = less[k0 + u];
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (k0 + u < n) {
+                S = l[u] == -1.0f ? own[u] : S + fmaf(l[u], S, own[u]);
+                ws[(k0 + u) * size] = S;
+            }
     }
 }
 
@@ -946,8 +971,8 @@ bool linear_attention_chunks_supported(const nb_linear_attention_desc_t &d) {
 }
 
 // Parts that the axis of tokens is cut into where there are fewer sequences and heads than SMs.  Cutting costs a pass for the
-// states (which loads keys and values again; about 0.6 of a chunk's time) and two launches; a CTA's own start and end are worth
-// about 5 chunks.
+// states (which loads keys and values again: 1.7 us a chunk of 128 x 128 heads, against 2.2) and two launches; a CTA's own start and
+// end are worth about 3 chunks.
 LinAttnSplit linear_attention_split(const nb_linear_attention_desc_t &d, int sms) {
     const long long bh = (long long)d.batch * d.heads;
     const int chunks = (d.time_steps + C - 1) / C;
@@ -957,7 +982,7 @@ LinAttnSplit linear_attention_split(const nb_linear_attention_desc_t &d, int sms
         const int per = (chunks + s - 1) / s;
         const int n = (chunks + per - 1) / per;         // what these parts come to
         const double waves = (double)((bh * n + sms - 1) / sms), pre = (double)((bh * (n - 1) + sms - 1) / sms);
-        const double cost = waves * (per + 5.0) + (n > 1 ? pre * (0.6 * per + 5.0) + 4.0 : 0.0);
+        const double cost = waves * (per + 3.0) + (n > 1 ? pre * (0.75 * per + 3.0) + 3.0 : 0.0);
         if (cost < least) {
             least = cost;
             best = {n, per};
@@ -977,6 +1002,9 @@ void linear_attention_chunks(nb_handle_s *h, const LinAttnParams &a, const LinAt
     p.ws = ws;
     p.ws_less = ws + (size_t)a.B * a.H * (split.n - 1) * a.dk * a.dv;
     p.status = h->d_status;
+    // Where not all CTAs run at once and lengths differ, a long sequence that starts late ends alone: 24 prompts of up to 1999 tokens took
+    // 66 to 78 us, by their order.
+    p.longest_first = (a.offsets || a.lengths) && split.n == 1 && a.B <= MAX_ORDERED && (long long)a.B * a.H > h->sm_count;
     p.scale = a.scale;
     p.log2_size = std::log2(std::fabs(a.scale));
     p.negative = a.scale < 0.0f;
