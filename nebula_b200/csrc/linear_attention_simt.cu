@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams
         for (int i = 0; i < 8; i++) {
             const float e = sums.since[row + i] ? 0.0f : expf(sums.hi[row + i]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) f[i][j] *= e;
+            for (int j = 0; j < 4; j++) f[i][j] = e == 0.0f ? 0.0f : f[i][j] * e;       // (what is forgotten may be infinite)
         }
         __syncthreads();
         load_tile<T>(K, v, a.v.token, w.n, v0, a.dv, p.vec[2]);
