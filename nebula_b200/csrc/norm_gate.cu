@@ -98,6 +98,10 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *red, int &tu
     float *r = red + (turn ^= 32);
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
+    if (lanes <= 256) {                     // at most eight warps
+        const float4 a = *(const float4 *)r, b = *(const float4 *)(r + 4);
+        return lanes == 64 ? a.x + a.y : lanes == 128 ? (a.x + a.y) + (a.z + a.w) : ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    }
     v = (threadIdx.x & 31) < (lanes >> 5) ? r[threadIdx.x & 31] : 0.0f;
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
     grid_begin();
     // the weights of both norms for a row of the tensors, four values of every vector after four of every vector
     extern __shared__ __align__(16) float smem[];
-    __shared__ float red[64];
+    __shared__ __align__(16) float red[64];
     const int lane = threadIdx.x & (p.lanes - 1), per_cta = blockDim.x / p.lanes;
     int turn = 0;
     const long long row0 = (long long)blockIdx.x * per_cta + threadIdx.x / p.lanes, pace = (long long)gridDim.x * per_cta;
@@ -157,20 +161,34 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         if (p.next_weight) smem[total + to] = p.next_weight[i];
     }
     __syncthreads();
-    // f *= by * weights
-    auto weigh = [&](float (&f)[V], const float *weights, int n, float by) {
-        const float *w = weights + (first / V + n * p.lanes + lane) * Q;
+    // A vector's values in pairs, two fp32 operations at once (V = 1: the second of the pair stays 0).
+    constexpr int H = V == 1 ? 1 : V / 2;
+    auto values = [](const auto &raw, float2 (&f)[H]) {
+        if constexpr (V == 1) f[0] = make_float2(raw.get(0), 0.0f);
+        else
 #pragma unroll
-        for (int i = 0; i < V; i += Q) {
-            if constexpr (V == 1) {
-                f[0] *= by * w[0];
-            } else {
+            for (int i = 0; i < H; i++) f[i] = make_float2(raw.get(2 * i), raw.get(2 * i + 1));
+    };
+    // f *= by * weights
+    auto weigh = [&](float2 (&f)[H], const float *weights, int n, float by) {
+        const float *w = weights + (first / V + n * p.lanes + lane) * Q;
+        if constexpr (V == 1) {
+            f[0].x *= by * w[0];
+        } else {
+            const float2 by2 = make_float2(by, by);
+#pragma unroll
+            for (int i = 0; i < V; i += Q) {
                 const float4 v = *(const float4 *)(w + i / Q * vecs * Q);
-                f[i] *= by * v.x;
-                f[i + 1] *= by * v.y;
-                f[i + 2] *= by * v.z;
-                f[i + 3] *= by * v.w;
+                f[i / 2] = mul2(mul2(f[i / 2], by2), make_float2(v.x, v.y));
+                f[i / 2 + 1] = mul2(mul2(f[i / 2 + 1], by2), make_float2(v.z, v.w));
             }
+        }
+    };
+    auto add_to = [&](float2 (&f)[H], const float *b, int c, const float *times) {      // f += scale * times * b
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            float &x = i & 1 ? f[i / 2].y : f[i / 2].x;
+            x = fmaf(load_now(b + first + c + i), times ? p.scale * load_now(times + first + c + i) : p.scale, x);
         }
     };
     Raw<T, V> x[NV], gate[GATE ? NV : 1];
@@ -189,36 +207,34 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         }
     };
     // of a row's values, subtracts the mean (of the layer norm) and returns 1 / the root of the mean square
-    auto spread = [&](float (&f)[NV][V], int mode) {
+    auto spread = [&](float2 (&f)[NV][H], int mode) {
         if (mode == NB_NORM_LAYER) {
-            float sum = 0.0f;
+            float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int n = 0; n < NV; n++)
 #pragma unroll
-                for (int i = 0; i < V; i++) sum += f[n][i];         // (columns past the last are zeros)
-            const float mean = row_sum(sum, p.lanes, red, turn) * p.by_width;
+                for (int i = 0; i < H; i++) sum = add2(sum, f[n][i]);       // (columns past the last are zeros)
+            const float mean = row_sum(sum.x + sum.y, p.lanes, red, turn) * p.by_width;
 #pragma unroll
             for (int n = 0; n < NV; n++)
                 if (in[n])
 #pragma unroll
-                    for (int i = 0; i < V; i++) f[n][i] -= mean;
+                    for (int i = 0; i < H; i++) f[n][i] = add2(f[n][i], make_float2(-mean, V == 1 ? 0.0f : -mean));
         }
-        float power = 0.0f;
+        float2 power = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int n = 0; n < NV; n++)
 #pragma unroll
-            for (int i = 0; i < V; i++) power = fmaf(f[n][i], f[n][i], power);
-        return inverse_root(fmaf(row_sum(power, p.lanes, red, turn), p.by_width, p.eps));
+            for (int i = 0; i < H; i++) power = fma2(f[n][i], f[n][i], power);
+        return inverse_root(fmaf(row_sum(power.x + power.y, p.lanes, red, turn), p.by_width, p.eps));
     };
     ask(row0 < p.rows);
     long long row = row0;
     for (long long base = (long long)blockIdx.x * per_cta; base < p.rows; base += pace) {
         const bool live = row < p.rows;
-        float f[NV][V];
+        float2 f[NV][H];
 #pragma unroll
-        for (int n = 0; n < NV; n++)
-#pragma unroll
-            for (int i = 0; i < V; i++) f[n][i] = x[n].get(i);
+        for (int n = 0; n < NV; n++) values(x[n], f[n]);
         Raw<T, V> z[GATE ? NV : 1];
         Raw<R, V> add[NV];
 #pragma unroll
@@ -235,17 +251,20 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
             if (!in[n]) continue;
             const unsigned c = (unsigned)((n * p.lanes + lane) * V);
             weigh(f[n], smem, n, by);
-            if (p.bias)
-#pragma unroll
-                for (int i = 0; i < V; i++)
-                    f[n][i] = fmaf(load_now(p.bias + first + c + i), p.channel_scale ? p.scale * load_now(p.channel_scale + first + c + i) : p.scale, f[n][i]);
+            if (p.bias) add_to(f[n], p.bias, c, p.channel_scale);
             if constexpr (GATE)
 #pragma unroll
-                for (int i = 0; i < V; i++) f[n][i] *= gate_value(z[n].get(i), p.gate_mode);
-            if (p.residual)
+                for (int i = 0; i < V; i++) {
+                    float &y = i & 1 ? f[n][i / 2].y : f[n][i / 2].x;
+                    y *= gate_value(z[n].get(i), p.gate_mode);
+                }
+            if (p.residual) {
+                float2 r[H];
+                values(add[n], r);
 #pragma unroll
-                for (int i = 0; i < V; i++) f[n][i] += add[n].get(i);
-            if (p.sum && live) put<R, V>(p.sum, os + c, f[n]);
+                for (int i = 0; i < H; i++) f[n][i] = add2(f[n][i], r[i]);
+            }
+            if (p.sum && live) put<R, V>(p.sum, os + c, (const float *)f[n]);
         }
         os += ds;
         if (p.next_norm != NB_NORM_NONE) {
@@ -258,12 +277,12 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
                     weigh(f[n], smem + total, n, by2);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < V; i++) f[n][i] *= by2;
+                    for (int i = 0; i < H; i++) f[n][i] = mul2(f[n][i], make_float2(by2, by2));
                 }
                 if (p.next_bias)
 #pragma unroll
-                    for (int i = 0; i < V; i++) f[n][i] += load_now(p.next_bias + first + c + i);
-                if (live) put<T, V>(p.y, oy + c, f[n]);
+                    for (int i = 0; i < V; i++) (i & 1 ? f[n][i / 2].y : f[n][i / 2].x) += load_now(p.next_bias + first + c + i);
+                if (live) put<T, V>(p.y, oy + c, (const float *)f[n]);
             }
         }
         oy += dy;
@@ -275,7 +294,7 @@ template <class T, class R, int V, int NV, bool GROUPED, bool GATE>
 __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
     grid_begin();
     extern __shared__ float smem[];         // GROUPED: a value per vector of the row, then one per group
-    __shared__ float red[64];
+    __shared__ __align__(16) float red[64];
     const int lane = threadIdx.x & (p.lanes - 1);
     int turn = 0;
     const long long row = (long long)blockIdx.x * (blockDim.x / p.lanes) + threadIdx.x / p.lanes;
