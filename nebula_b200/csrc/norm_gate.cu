@@ -26,8 +26,9 @@ struct NormParams {
     long long rows;
     int width, groups;          // of a row; groups > 1 only in the general kernel
     int fold;                   // > 0: a row here is one of `fold` groups of a row of the tensors
+    int joined;                 // with fold: a CTA has all groups of a row, and the second norm is over them
     int norm, next_norm, gate_mode;
-    float eps, scale, by_width, by_group;       // by_...: 1 / the values of a row, of a group
+    float eps, scale, by_width, by_group, by_next;      // by_...: 1 / the values of a row, of a group, of what the second norm is over
     int lanes;                  // threads of a row, a power of two
 };
 
@@ -90,19 +91,23 @@ template <int V> __device__ __forceinline__ void weights_at(const float *w, int 
         }
 }
 
-// Sum over the threads of a row, the same for all of them.  Rows of up to a warp are segments of one; wider ones are a CTA of their
-// own, whose warps' sums are added in order.  `red` has a half for each of two sums in turn, so that one barrier a sum is enough.
+// Sum over the threads of a row, `lanes` of them from a multiple of that on, the same for all.  Up to a warp (a power of two) they are a
+// segment of one; else their warps' sums are added in order.  `red` has a half for each of two sums in turn, so that one barrier
+// a sum is enough.
 __device__ __forceinline__ float row_sum(float v, int lanes, float *red, int &turn) {
     for (int o = min(lanes, 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lanes <= 32) return v;
     float *r = red + (turn ^= 32);
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    if (lanes <= 256) {                     // at most eight warps
-        const float4 a = *(const float4 *)r, b = *(const float4 *)(r + 4);
-        return lanes == 64 ? a.x + a.y : lanes == 128 ? (a.x + a.y) + (a.z + a.w) : ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    const int warps = lanes >> 5;
+    r += threadIdx.x / lanes * warps;
+    if (warps <= 8) {
+        v = r[0] + r[1];
+        for (int i = 2; i < warps; i++) v += r[i];
+        return v;
     }
-    v = (threadIdx.x & 31) < (lanes >> 5) ? r[threadIdx.x & 31] : 0.0f;
+    v = (threadIdx.x & 31) < warps ? r[threadIdx.x & 31] : 0.0f;
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
@@ -207,14 +212,14 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         }
     };
     // of a row's values, subtracts the mean (of the layer norm) and returns 1 / the root of the mean square
-    auto spread = [&](float2 (&f)[NV][H], int mode) {
+    auto spread = [&](float2 (&f)[NV][H], int mode, int lanes, float by_width) {
         if (mode == NB_NORM_LAYER) {
             float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int n = 0; n < NV; n++)
 #pragma unroll
                 for (int i = 0; i < H; i++) sum = add2(sum, f[n][i]);       // (columns past the last are zeros)
-            const float mean = row_sum(sum.x + sum.y, p.lanes, red, turn) * p.by_width;
+            const float mean = row_sum(sum.x + sum.y, lanes, red, turn) * by_width;
 #pragma unroll
             for (int n = 0; n < NV; n++)
                 if (in[n])
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         for (int n = 0; n < NV; n++)
 #pragma unroll
             for (int i = 0; i < H; i++) power = fma2(f[n][i], f[n][i], power);
-        return inverse_root(fmaf(row_sum(power.x + power.y, p.lanes, red, turn), p.by_width, p.eps));
+        return inverse_root(fmaf(row_sum(power.x + power.y, lanes, red, turn), by_width, p.eps));
     };
     ask(row0 < p.rows);
     long long row = row0;
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         row += pace;
         ox += dx, og += dg, orr += dr;
         if (base + pace < p.rows) ask(row < p.rows);
-        const float by = p.norm != NB_NORM_NONE ? spread(f, p.norm) : 1.0f;
+        const float by = p.norm != NB_NORM_NONE ? spread(f, p.norm, p.lanes, p.by_width) : 1.0f;
 #pragma unroll
         for (int n = 0; n < NV; n++) {
             if (!in[n]) continue;
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         }
         os += ds;
         if (p.next_norm != NB_NORM_NONE) {
-            const float by2 = spread(f, p.next_norm);
+            const float by2 = spread(f, p.next_norm, p.joined ? blockDim.x : p.lanes, p.by_next);
 #pragma unroll
             for (int n = 0; n < NV; n++) {
                 if (!in[n]) continue;
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
     }
 }
 
-// The others: wide rows, rows whose groups a second norm joins (GROUPED), tensors of more than 2^32 values.  GATE: there is a gate.
+// The others: wide rows, wide ones whose groups a second norm joins (GROUPED), tensors of more than 2^32 values.  GATE: there is a gate.
 template <class T, class R, int V, int NV, bool GROUPED, bool GATE>
 __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
     grid_begin();
@@ -445,7 +450,7 @@ void launch_general(nb_handle_s *h, const NormParams &p) {
 template <class T, class R, int V, int NV, bool GATE>
 bool launch_rows(nb_handle_s *h, const NormParams &p) {
     auto kernel = norm_gate_rows_kernel<T, R, V, NV, GATE>;
-    const int tpb = p.lanes > 32 ? p.lanes : 256, per_cta = tpb / p.lanes;
+    const int tpb = p.joined ? p.lanes * p.fold : p.lanes > 32 ? p.lanes : 256, per_cta = tpb / p.lanes;
     const int total = std::max(p.fold, 1) * p.width;
     const size_t smem = (size_t)total * (p.next_weight ? 2 : 1) * sizeof(float);
     if (smem > 48 * 1024) return false;
@@ -466,21 +471,40 @@ bool launch_rows(nb_handle_s *h, const NormParams &p) {
 
 constexpr int MAX_WIDTH = 32768;        // 1024 threads with 32 values each
 
-// Threads and accesses of a row: two accesses a thread, or one while the rows are too few to fill the device and a row's
-// latency counts; more where 1024 threads do not hold it.  wide: offsets need 64 bits.
+// Threads and accesses of a row: two accesses a thread (eight of single values), or one while the rows are too few to fill the device
+// and a row's latency counts; more where 1024 threads do not hold it.  wide: offsets need 64 bits.
 template <class T, class R, int V>
 void choose(nb_handle_s *h, NormParams p, bool wide) {
-    const int vecs = (p.width + V - 1) / V;
-    const int want = p.rows * 2 <= h->sm_count ? 1 : 2;
-    int lanes = p.groups > 1 ? 64 : 4;
-    while (lanes < 1024 && lanes * want < vecs) lanes *= 2;
-    p.lanes = lanes;
-    const int nv = (vecs + lanes - 1) / lanes;
-    if (p.groups == 1 && lanes <= 256 && nv <= 2 && !wide) {
-        const bool done = nv <= 1 ? p.gate ? launch_rows<T, R, V, 1, true>(h, p) : launch_rows<T, R, V, 1, false>(h, p)
-                                  : p.gate ? launch_rows<T, R, V, 2, true>(h, p) : launch_rows<T, R, V, 2, false>(h, p);
-        if (done) return;
+    const int few = p.rows * 2 <= h->sm_count;
+    constexpr int MANY = V == 1 ? 8 : 2;        // accesses of a thread
+    auto lanes_for = [&](int width, int want, int least) {
+        const int vecs = (width + V - 1) / V;
+        int lanes = least;
+        while (lanes < 1024 && lanes * want < vecs) lanes *= 2;
+        return lanes;
+    };
+    if (!wide) {
+        NormParams r = p;
+        if (p.groups > 1) {                     // joined by the second norm
+            r.fold = p.groups;
+            r.joined = 1;
+            r.rows *= p.groups;
+            r.width /= p.groups;
+            r.by_width = p.by_group;
+            r.groups = 1;
+        }
+        for (int want : {1, MANY}) {
+            if (want == 1 && !few) continue;
+            r.lanes = lanes_for(r.width, want, 4);
+            const int tpb = r.joined ? r.lanes * r.fold : r.lanes, nv = ((r.width + V - 1) / V + r.lanes - 1) / r.lanes;
+            if (tpb > 256 || nv > want || (r.joined && tpb % 32)) continue;
+            const bool done = want == 1 ? p.gate ? launch_rows<T, R, V, 1, true>(h, r) : launch_rows<T, R, V, 1, false>(h, r)
+                                        : p.gate ? launch_rows<T, R, V, MANY, true>(h, r) : launch_rows<T, R, V, MANY, false>(h, r);
+            if (done) return;
+        }
     }
+    p.lanes = lanes_for(p.width, few ? 1 : 2, p.groups > 1 ? 64 : 4);
+    const int nv = ((p.width + V - 1) / V + p.lanes - 1) / p.lanes;
     auto go = [&](auto accesses) {
         constexpr int NV = decltype(accesses)::value;
         if (p.groups > 1) {
@@ -550,6 +574,7 @@ void launch_norm_gate(nb_handle_s *h, const nb_norm_gate_desc_t &d, const nb_nor
     }
     p.by_width = 1.0f / p.width;
     p.by_group = (float)p.groups / p.width;
+    p.by_next = 1.0f / p.width;
     // whole accesses of 16 bytes: every row, group and vector of weights starts on such a boundary and is made of whole ones
     const int v = d.dtype == NB_DTYPE_BF16 ? 8 : 4;
     const bool whole = align % 16 == 0 && p.width % v == 0 && p.width / p.groups % v == 0;
