@@ -69,6 +69,7 @@ class LinearAttentionDesc(C.Structure):
 _ATTENTION_IO = struct.Struct("=27q")
 _NORM_DESC = struct.Struct("=8i2f5q")
 _NORM_IO = struct.Struct("=10q")
+_NORM_CALL = struct.Struct("=8i2f5q10q")     # one behind the other
 
 
 class ConvFusion(C.Structure):
@@ -202,21 +203,14 @@ def _mem(t):
     return MEM_DEVICE if t.is_cuda else MEM_HOST
 
 
-# Checks of the calls that a server makes for every token, where the binding's own time counts.
-_torch = None
+# Checks of the calls that a server makes for every token, where the binding's own time counts.  torch is imported with the first.
+_F32 = _BF16 = _I32 = _empty_like = None
 
 
-def _kind(dtype):
-    """nb_dtype of a torch dtype, -1 for another one."""
-    global _torch
-    if _torch is None:
-        import torch
-        _torch = torch
-    return 0 if dtype is _torch.float32 else 1 if dtype is _torch.bfloat16 else -1
-
-
-def _empty_like(t):
-    return _torch.empty_like(t, memory_format=_torch.contiguous_format)
+def _torch_types():
+    global _F32, _BF16, _I32, _empty_like
+    import torch
+    _F32, _BF16, _I32, _empty_like = torch.float32, torch.bfloat16, torch.int32, torch.empty_like
 
 
 def _rows(t, shape, dtype, width):
@@ -231,10 +225,13 @@ def _rows(t, shape, dtype, width):
     raise NebulaError(1, "norm: rows are contiguous, and evenly spaced in two dimensions")
 
 
+def _new_rows(t):
+    """A contiguous tensor like t."""
+    return _empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _weights(t, width):
-    if t is None:
-        return 0
-    if t.dtype is not _torch.float32 or t.numel() != width or not t.is_contiguous() or not t.is_cuda:
+    if t.dtype is not _F32 or t.numel() != width or not t.is_contiguous() or not t.is_cuda:
         raise NebulaError(1, "norm: weights are contiguous float32 tensors of the row's width on the device")
     return t.data_ptr()
 
@@ -251,7 +248,9 @@ class Handle:
         if rc != 0:
             raise NebulaError(rc, (self.lib.nb_last_error(None) or b"").decode())
         self.h = h
-        self._norm_desc, self._norm_io = (C.c_char * _NORM_DESC.size)(), (C.c_char * _NORM_IO.size)()
+        self._norm = (C.c_char * _NORM_CALL.size)()
+        self._norm_desc = C.addressof(self._norm)
+        self._norm_io = self._norm_desc + _NORM_DESC.size
         self.set_math(math)
 
     def check(self, rc):
@@ -353,25 +352,38 @@ class Handle:
         """s = residual + scale * channel_scale * (norm(x) * gate function(gate)) and y = next_norm(s), row by row
         (nb_norm_gate_residual); x [..., width], float32 or bfloat16, rows evenly spaced.  Returns (s, y), y None without a second
         norm.  `out` may be the residual itself, and `y` x itself."""
+        if _F32 is None:
+            _torch_types()
         shape, dtype = x.shape, x.dtype
-        kind = _kind(dtype)
-        if kind < 0 or not x.is_cuda:
+        kind = 1 if dtype is _BF16 else 0 if dtype is _F32 else -1
+        if kind < 0:
             raise NebulaError(1, "norm: x is a float32 or bfloat16 tensor on the device")
         width = shape[-1]
-        like = x if residual is None else residual
-        if out is None:
-            out = _empty_like(like)
-        if y is None and next_norm != "none":
-            y = _empty_like(x)
         px, sx = _rows(x, shape, dtype, width)
         pg, sg = (0, 0) if gate is None else _rows(gate, shape, dtype, width)
-        pr, sr = (0, 0) if residual is None else _rows(residual, shape, residual.dtype, width)
-        po, so = _rows(out, shape, like.dtype, width)
-        py, sy = (0, 0) if y is None else _rows(y, shape, dtype, width)
-        _NORM_DESC.pack_into(self._norm_desc, 0, x.numel() // width if width else 0, width, groups, NORMS[norm], NORMS[next_norm],
-                             GATES[gate_act] if gate is not None else 0, kind, _kind(like.dtype), eps, scale, sx, sg, sr, so, sy)
-        _NORM_IO.pack_into(self._norm_io, 0, px, _weights(weight, width), _weights(bias, width), pg, _weights(channel_scale, width), pr, po,
-                           _weights(next_weight, width), _weights(next_bias, width), py)
+        if residual is None:
+            pr = sr = 0
+            like, rkind = x, kind
+        else:
+            like, rdtype = residual, residual.dtype
+            rkind = 1 if rdtype is _BF16 else 0 if rdtype is _F32 else -1
+            pr, sr = _rows(residual, shape, rdtype, width)
+        if out is None:
+            out = _new_rows(like)
+            po, so = out.data_ptr(), width
+        else:
+            po, so = _rows(out, shape, like.dtype, width)
+        py = sy = 0
+        if y is not None:
+            py, sy = _rows(y, shape, dtype, width)
+        elif next_norm != "none":
+            y = _new_rows(x)
+            py, sy = y.data_ptr(), width
+        _NORM_CALL.pack_into(
+            self._norm, 0, x.numel() // width if width else 0, width, groups, NORMS[norm], NORMS[next_norm], 0 if gate is None else GATES[gate_act],
+            kind, rkind, eps, scale, sx, sg, sr, so, sy, px, 0 if weight is None else _weights(weight, width),
+            0 if bias is None else _weights(bias, width), pg, 0 if channel_scale is None else _weights(channel_scale, width), pr, po,
+            0 if next_weight is None else _weights(next_weight, width), 0 if next_bias is None else _weights(next_bias, width), py)
         rc = self.lib.nb_norm_gate_residual(self.h, self._norm_desc, self._norm_io)
         if rc:
             self.check(rc)
@@ -530,11 +542,15 @@ class LinearAttention(_Plan):
         self.desc = LinearAttentionDesc(batch, time_steps, heads, key_heads or heads, key_dim, value_dim, DTYPES[dtype], scale)
         handle.check(handle.lib.nb_linear_attention_plan_create(handle.h, C.byref(self.desc), C.byref(self.p)))
         self.dtype = torch.float32 if dtype == "f32" else torch.bfloat16
-        _kind(self.dtype)
+        if _F32 is None:
+            _torch_types()
+        self._empty = torch.empty
         self._state = (heads, key_dim, value_dim)
         self._whole = self._shapes((batch, time_steps))
         self._single = self._shapes((batch,))
-        self._io = (C.c_char * _ATTENTION_IO.size)()
+        self._buffer = (C.c_char * _ATTENTION_IO.size)()
+        self._io = C.addressof(self._buffer)
+        self._states = (batch, *self._state)
 
     def _shapes(self, lead):
         """Of q and k, of v and the result, of the log decays."""
@@ -553,7 +569,7 @@ class LinearAttention(_Plan):
     def _decay(self, g, shape):
         if g is None:
             return 0, 0, 0, 0
-        if g.dtype is _torch.float32 and g.is_cuda:
+        if g.dtype is _F32 and g.is_cuda:
             if g.shape == shape:
                 st = g.stride()
                 return (g.data_ptr(), st[0], st[1], st[2]) if len(st) == 3 else (g.data_ptr(), st[0], st[0], st[1])
@@ -562,31 +578,31 @@ class LinearAttention(_Plan):
         raise NebulaError(1, f"linear attention: log_decay is {tuple(g.shape)} {g.dtype}, expected float32 {shape} or {shape[-1:]} on the device")
 
     def _ints(self, t, n, what):
-        if t is None:
-            return 0
-        if t.dtype is not _torch.int32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
+        if t.dtype is not _I32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
             raise NebulaError(1, f"linear attention: {what} is a contiguous int32 tensor of {n} values on the device")
         return t.data_ptr()
 
-    def _pool(self, t, slots, what):
-        if t is None:
-            return 0
-        if t.dtype is not _torch.float32 or t.shape != (slots, *self._state) or not t.is_contiguous() or not t.is_cuda:
-            raise NebulaError(1, f"linear attention: {what} is a contiguous float32 tensor {(slots, *self._state)} on the device")
+    def _pool(self, t, shape, what):
+        if t.dtype is not _F32 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
+            raise NebulaError(1, f"linear attention: {what} is a contiguous float32 tensor {shape} on the device")
         return t.data_ptr()
 
     def _run(self, fn, shapes, q, k, v, log_decay, state, state_out, offsets, lengths, slots, out):
         keys, values, decays = shapes
         if out is None:
-            out = _torch.empty(values, device=v.device, dtype=self.dtype)
-        batch = self.desc.batch
-        pool = state if state is not None else state_out
-        n = pool.shape[0] if pool is not None and slots is not None else batch
+            out = self._empty(values, device=v.device, dtype=self.dtype)
+        states = self._states
+        if slots is not None:
+            pool = state if state is not None else state_out
+            if pool is not None:
+                states = (pool.shape[0], *self._state)
+        batch = self._states[0]
         _ATTENTION_IO.pack_into(
-            self._io, 0, *self._view(q, keys, "q"), *self._view(k, keys, "k"), *self._view(v, values, "v"), *self._decay(log_decay, decays),
-            *self._view(out, values, "out"), self._ints(offsets, batch + 1, "offsets"), self._ints(lengths, batch, "lengths"),
-            values[0] if offsets is not None else 0, self._pool(state, n, "state"), self._pool(state_out, n, "state_out"),
-            self._ints(slots, batch, "slots"), n)
+            self._buffer, 0, *self._view(q, keys, "q"), *self._view(k, keys, "k"), *self._view(v, values, "v"), *self._decay(log_decay, decays),
+            *self._view(out, values, "out"), 0 if offsets is None else self._ints(offsets, batch + 1, "offsets"),
+            0 if lengths is None else self._ints(lengths, batch, "lengths"), 0 if offsets is None else values[0],
+            0 if state is None else self._pool(state, states, "state"), 0 if state_out is None else self._pool(state_out, states, "state_out"),
+            0 if slots is None else self._ints(slots, batch, "slots"), states[0])
         rc = fn(self.p, self._io)
         if rc:
             self.handle.check(rc)

@@ -26,9 +26,8 @@ struct NormParams {
     long long rows;
     int width, groups;          // of a row; groups > 1 only in the general kernel
     int fold;                   // > 0: a row here is one of `fold` groups of a row of the tensors
-    int joined;                 // with fold: a CTA has all groups of a row, and the second norm is over them
     int norm, next_norm, gate_mode;
-    float eps, scale, by_width, by_group, by_next;      // by_...: 1 / the values of a row, of a group, of what the second norm is over
+    float eps, scale, by_width, by_group;       // by_...: 1 / the values of a row, of a group
     int lanes;                  // threads of a row, a power of two
 };
 
@@ -91,23 +90,15 @@ template <int V> __device__ __forceinline__ void weights_at(const float *w, int 
         }
 }
 
-// Sum over the threads of a row, `lanes` of them from a multiple of that on, the same for all.  Up to a warp (a power of two) they are a
-// segment of one; else their warps' sums are added in order.  `red` has a half for each of two sums in turn, so that one barrier
-// a sum is enough.
+// Sum over the threads of a row, the same for all of them.  Rows of up to a warp are segments of one; wider ones are a CTA of their
+// own, whose warps' sums are added in order.  `red` has a half for each of two sums in turn, so that one barrier a sum is enough.
 __device__ __forceinline__ float row_sum(float v, int lanes, float *red, int &turn) {
     for (int o = min(lanes, 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lanes <= 32) return v;
     float *r = red + (turn ^= 32);
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    const int warps = lanes >> 5;
-    r += threadIdx.x / lanes * warps;
-    if (warps <= 8) {
-        v = r[0] + r[1];
-        for (int i = 2; i < warps; i++) v += r[i];
-        return v;
-    }
-    v = (threadIdx.x & 31) < warps ? r[threadIdx.x & 31] : 0.0f;
+    v = (threadIdx.x & 31) < (lanes >> 5) ? r[threadIdx.x & 31] : 0.0f;
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
@@ -145,7 +136,7 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
     grid_begin();
     // the weights of both norms for a row of the tensors, four values of every vector after four of every vector
     extern __shared__ __align__(16) float smem[];
-    __shared__ __align__(16) float red[64];
+    __shared__ float red[64];
     const int lane = threadIdx.x & (p.lanes - 1), per_cta = blockDim.x / p.lanes;
     int turn = 0;
     const long long row0 = (long long)blockIdx.x * per_cta + threadIdx.x / p.lanes, pace = (long long)gridDim.x * per_cta;
@@ -166,34 +157,20 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         if (p.next_weight) smem[total + to] = p.next_weight[i];
     }
     __syncthreads();
-    // A vector's values in pairs, two fp32 operations at once (V = 1: the second of the pair stays 0).
-    constexpr int H = V == 1 ? 1 : V / 2;
-    auto values = [](const auto &raw, float2 (&f)[H]) {
-        if constexpr (V == 1) f[0] = make_float2(raw.get(0), 0.0f);
-        else
-#pragma unroll
-            for (int i = 0; i < H; i++) f[i] = make_float2(raw.get(2 * i), raw.get(2 * i + 1));
-    };
     // f *= by * weights
-    auto weigh = [&](float2 (&f)[H], const float *weights, int n, float by) {
+    auto weigh = [&](float (&f)[V], const float *weights, int n, float by) {
         const float *w = weights + (first / V + n * p.lanes + lane) * Q;
-        if constexpr (V == 1) {
-            f[0].x *= by * w[0];
-        } else {
-            const float2 by2 = make_float2(by, by);
 #pragma unroll
-            for (int i = 0; i < V; i += Q) {
+        for (int i = 0; i < V; i += Q) {
+            if constexpr (V == 1) {
+                f[0] *= by * w[0];
+            } else {
                 const float4 v = *(const float4 *)(w + i / Q * vecs * Q);
-                f[i / 2] = mul2(mul2(f[i / 2], by2), make_float2(v.x, v.y));
-                f[i / 2 + 1] = mul2(mul2(f[i / 2 + 1], by2), make_float2(v.z, v.w));
+                f[i] *= by * v.x;
+                f[i + 1] *= by * v.y;
+                f[i + 2] *= by * v.z;
+                f[i + 3] *= by * v.w;
             }
-        }
-    };
-    auto add_to = [&](float2 (&f)[H], const float *b, int c, const float *times) {      // f += scale * times * b
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            float &x = i & 1 ? f[i / 2].y : f[i / 2].x;
-            x = fmaf(load_now(b + first + c + i), times ? p.scale * load_now(times + first + c + i) : p.scale, x);
         }
     };
     Raw<T, V> x[NV], gate[GATE ? NV : 1];
@@ -212,34 +189,36 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         }
     };
     // of a row's values, subtracts the mean (of the layer norm) and returns 1 / the root of the mean square
-    auto spread = [&](float2 (&f)[NV][H], int mode, int lanes, float by_width) {
+    auto spread = [&](float (&f)[NV][V], int mode) {
         if (mode == NB_NORM_LAYER) {
-            float2 sum = make_float2(0.0f, 0.0f);
+            float sum = 0.0f;
 #pragma unroll
             for (int n = 0; n < NV; n++)
 #pragma unroll
-                for (int i = 0; i < H; i++) sum = add2(sum, f[n][i]);       // (columns past the last are zeros)
-            const float mean = row_sum(sum.x + sum.y, lanes, red, turn) * by_width;
+                for (int i = 0; i < V; i++) sum += f[n][i];         // (columns past the last are zeros)
+            const float mean = row_sum(sum, p.lanes, red, turn) * p.by_width;
 #pragma unroll
             for (int n = 0; n < NV; n++)
                 if (in[n])
 #pragma unroll
-                    for (int i = 0; i < H; i++) f[n][i] = add2(f[n][i], make_float2(-mean, V == 1 ? 0.0f : -mean));
+                    for (int i = 0; i < V; i++) f[n][i] -= mean;
         }
-        float2 power = make_float2(0.0f, 0.0f);
+        float power = 0.0f;
 #pragma unroll
         for (int n = 0; n < NV; n++)
 #pragma unroll
-            for (int i = 0; i < H; i++) power = fma2(f[n][i], f[n][i], power);
-        return inverse_root(fmaf(row_sum(power.x + power.y, lanes, red, turn), by_width, p.eps));
+            for (int i = 0; i < V; i++) power = fmaf(f[n][i], f[n][i], power);
+        return inverse_root(fmaf(row_sum(power, p.lanes, red, turn), p.by_width, p.eps));
     };
     ask(row0 < p.rows);
     long long row = row0;
     for (long long base = (long long)blockIdx.x * per_cta; base < p.rows; base += pace) {
         const bool live = row < p.rows;
-        float2 f[NV][H];
+        float f[NV][V];
 #pragma unroll
-        for (int n = 0; n < NV; n++) values(x[n], f[n]);
+        for (int n = 0; n < NV; n++)
+#pragma unroll
+            for (int i = 0; i < V; i++) f[n][i] = x[n].get(i);
         Raw<T, V> z[GATE ? NV : 1];
         Raw<R, V> add[NV];
 #pragma unroll
@@ -250,30 +229,27 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
         row += pace;
         ox += dx, og += dg, orr += dr;
         if (base + pace < p.rows) ask(row < p.rows);
-        const float by = p.norm != NB_NORM_NONE ? spread(f, p.norm, p.lanes, p.by_width) : 1.0f;
+        const float by = p.norm != NB_NORM_NONE ? spread(f, p.norm) : 1.0f;
 #pragma unroll
         for (int n = 0; n < NV; n++) {
             if (!in[n]) continue;
             const unsigned c = (unsigned)((n * p.lanes + lane) * V);
             weigh(f[n], smem, n, by);
-            if (p.bias) add_to(f[n], p.bias, c, p.channel_scale);
+            if (p.bias)
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    f[n][i] = fmaf(load_now(p.bias + first + c + i), p.channel_scale ? p.scale * load_now(p.channel_scale + first + c + i) : p.scale, f[n][i]);
             if constexpr (GATE)
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    float &y = i & 1 ? f[n][i / 2].y : f[n][i / 2].x;
-                    y *= gate_value(z[n].get(i), p.gate_mode);
-                }
-            if (p.residual) {
-                float2 r[H];
-                values(add[n], r);
+                for (int i = 0; i < V; i++) f[n][i] *= gate_value(z[n].get(i), p.gate_mode);
+            if (p.residual)
 #pragma unroll
-                for (int i = 0; i < H; i++) f[n][i] = add2(f[n][i], r[i]);
-            }
-            if (p.sum && live) put<R, V>(p.sum, os + c, (const float *)f[n]);
+                for (int i = 0; i < V; i++) f[n][i] += add[n].get(i);
+            if (p.sum && live) put<R, V>(p.sum, os + c, f[n]);
         }
         os += ds;
         if (p.next_norm != NB_NORM_NONE) {
-            const float by2 = spread(f, p.next_norm, p.joined ? blockDim.x : p.lanes, p.by_next);
+            const float by2 = spread(f, p.next_norm);
 #pragma unroll
             for (int n = 0; n < NV; n++) {
                 if (!in[n]) continue;
@@ -282,24 +258,24 @@ __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
                     weigh(f[n], smem + total, n, by2);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < H; i++) f[n][i] = mul2(f[n][i], make_float2(by2, by2));
+                    for (int i = 0; i < V; i++) f[n][i] *= by2;
                 }
                 if (p.next_bias)
 #pragma unroll
-                    for (int i = 0; i < V; i++) (i & 1 ? f[n][i / 2].y : f[n][i / 2].x) += load_now(p.next_bias + first + c + i);
-                if (live) put<T, V>(p.y, oy + c, (const float *)f[n]);
+                    for (int i = 0; i < V; i++) f[n][i] += load_now(p.next_bias + first + c + i);
+                if (live) put<T, V>(p.y, oy + c, f[n]);
             }
         }
         oy += dy;
     }
 }
 
-// The others: wide rows, wide ones whose groups a second norm joins (GROUPED), tensors of more than 2^32 values.  GATE: there is a gate.
+// The others: wide rows, rows whose groups a second norm joins (GROUPED), tensors of more than 2^32 values.  GATE: there is a gate.
 template <class T, class R, int V, int NV, bool GROUPED, bool GATE>
 __global__ void __launch_bounds__(1024) norm_gate_kernel(NormParams p) {
     grid_begin();
     extern __shared__ float smem[];         // GROUPED: a value per vector of the row, then one per group
-    __shared__ __align__(16) float red[64];
+    __shared__ float red[64];
     const int lane = threadIdx.x & (p.lanes - 1);
     int turn = 0;
     const long long row = (long long)blockIdx.x * (blockDim.x / p.lanes) + threadIdx.x / p.lanes;
@@ -450,7 +426,7 @@ void launch_general(nb_handle_s *h, const NormParams &p) {
 template <class T, class R, int V, int NV, bool GATE>
 bool launch_rows(nb_handle_s *h, const NormParams &p) {
     auto kernel = norm_gate_rows_kernel<T, R, V, NV, GATE>;
-    const int tpb = p.joined ? p.lanes * p.fold : p.lanes > 32 ? p.lanes : 256, per_cta = tpb / p.lanes;
+    const int tpb = p.lanes > 32 ? p.lanes : 256, per_cta = tpb / p.lanes;
     const int total = std::max(p.fold, 1) * p.width;
     const size_t smem = (size_t)total * (p.next_weight ? 2 : 1) * sizeof(float);
     if (smem > 48 * 1024) return false;
@@ -471,40 +447,21 @@ bool launch_rows(nb_handle_s *h, const NormParams &p) {
 
 constexpr int MAX_WIDTH = 32768;        // 1024 threads with 32 values each
 
-// Threads and accesses of a row: two accesses a thread (eight of single values), or one while the rows are too few to fill the device
-// and a row's latency counts; more where 1024 threads do not hold it.  wide: offsets need 64 bits.
+// Threads and accesses of a row: two accesses a thread, or one while the rows are too few to fill the device and a row's
+// latency counts; more where 1024 threads do not hold it.  wide: offsets need 64 bits.
 template <class T, class R, int V>
 void choose(nb_handle_s *h, NormParams p, bool wide) {
-    const int few = p.rows * 2 <= h->sm_count;
-    constexpr int MANY = V == 1 ? 8 : 2;        // accesses of a thread
-    auto lanes_for = [&](int width, int want, int least) {
-        const int vecs = (width + V - 1) / V;
-        int lanes = least;
-        while (lanes < 1024 && lanes * want < vecs) lanes *= 2;
-        return lanes;
-    };
-    if (!wide) {
-        NormParams r = p;
-        if (p.groups > 1) {                     // joined by the second norm
-            r.fold = p.groups;
-            r.joined = 1;
-            r.rows *= p.groups;
-            r.width /= p.groups;
-            r.by_width = p.by_group;
-            r.groups = 1;
-        }
-        for (int want : {1, MANY}) {
-            if (want == 1 && !few) continue;
-            r.lanes = lanes_for(r.width, want, 4);
-            const int tpb = r.joined ? r.lanes * r.fold : r.lanes, nv = ((r.width + V - 1) / V + r.lanes - 1) / r.lanes;
-            if (tpb > 256 || nv > want || (r.joined && tpb % 32)) continue;
-            const bool done = want == 1 ? p.gate ? launch_rows<T, R, V, 1, true>(h, r) : launch_rows<T, R, V, 1, false>(h, r)
-                                        : p.gate ? launch_rows<T, R, V, MANY, true>(h, r) : launch_rows<T, R, V, MANY, false>(h, r);
-            if (done) return;
-        }
+    const int vecs = (p.width + V - 1) / V;
+    const int want = p.rows * 2 <= h->sm_count ? 1 : 2;
+    int lanes = p.groups > 1 ? 64 : 4;
+    while (lanes < 1024 && lanes * want < vecs) lanes *= 2;
+    p.lanes = lanes;
+    const int nv = (vecs + lanes - 1) / lanes;
+    if (p.groups == 1 && lanes <= 256 && nv <= 2 && !wide) {
+        const bool done = nv <= 1 ? p.gate ? launch_rows<T, R, V, 1, true>(h, p) : launch_rows<T, R, V, 1, false>(h, p)
+                                  : p.gate ? launch_rows<T, R, V, 2, true>(h, p) : launch_rows<T, R, V, 2, false>(h, p);
+        if (done) return;
     }
-    p.lanes = lanes_for(p.width, few ? 1 : 2, p.groups > 1 ? 64 : 4);
-    const int nv = ((p.width + V - 1) / V + p.lanes - 1) / p.lanes;
     auto go = [&](auto accesses) {
         constexpr int NV = decltype(accesses)::value;
         if (p.groups > 1) {
@@ -574,7 +531,6 @@ void launch_norm_gate(nb_handle_s *h, const nb_norm_gate_desc_t &d, const nb_nor
     }
     p.by_width = 1.0f / p.width;
     p.by_group = (float)p.groups / p.width;
-    p.by_next = 1.0f / p.width;
     // whole accesses of 16 bytes: every row, group and vector of weights starts on such a boundary and is made of whole ones
     const int v = d.dtype == NB_DTYPE_BF16 ? 8 : 4;
     const bool whole = align % 16 == 0 && p.width % v == 0 && p.width / p.groups % v == 0;
