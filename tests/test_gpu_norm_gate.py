@@ -64,6 +64,18 @@ def test_norms(handle, case, types):
         assert rel(y, wanty) <= TOL[dtype]
 
 
+@pytest.mark.parametrize("types", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("case", [
+    (300, 866, 1, "rms", "silu", True, "none"), (300, 867, 1, "layer", "silu", True, "rms"), (301, 2046, 1, "rms", None, True, "layer"),
+    (301, 2050, 1, "rms", "sigmoid", True, "rms"), (200, 2047, 1, "layer", None, False, "none"), (200, 2049, 1, "rms", "linear", True, "rms"),
+    (300, 2, 1, "rms", None, True, "rms"), (300, 6, 3, "layer", "silu", True, "rms"), (200, 6, 2, "rms", None, True, "rms"),
+    (150, 1000, 100, "rms", "silu", True, "layer"), (80, 32766, 1, "layer", "silu", True, "rms"),
+])
+def test_rows_in_pairs_and_single_values(handle, case, types):
+    """Widths that are not whole 16-byte accesses, with enough rows that a thread has several."""
+    test_norms(handle, case, types)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("width,skip", [(512, 0), (512, 8), (512, 3), (100, 1)])
 def test_strided_rows_and_in_place(handle, width, skip, dtype):
