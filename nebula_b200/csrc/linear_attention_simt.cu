@@ -5,7 +5,9 @@
 //   3. out_i = scale * [ sum_{j<=i} exp(G_ij) (q_i . k_j) v_j + exp(G_i) q_i^T S_c ].
 // Bound by fp32 arithmetic (C (dk + dv) / 2 + 2 dk dv FMAs a token and head): a thread has 8 x 4 values of a 64 x 64 product, so that
 // three 16-byte reads of shared memory feed 32 FMAs, from tiles that lie as the tensors do (with transposed copies and 4-byte loads
-// 4 x 1023 tokens, 8 heads of 64 took 71 us, most of it waiting for loads).
+// 4 x 1023 tokens, 8 heads of 64 took 71 us, most of it waiting for loads; now 49 to 52, of which the outputs are 31, with half of the
+// issue slots used and an SM's four CTAs in one wave).  Transposed tiles, which let two fp32 operations go at once, took 59: their
+// loads touch twice the lines.  Products go as far as a head's values: 16 heads of 32, 10 x 3031 tokens 451 -> 357 us.
 // G, the sums of log decays, are kept to 48 bits (two fp32 numbers), because the weight of two late tokens of a chunk is the
 // difference of two large sums.  A product with a masked weight of zero is NaN where v is not finite: the first launch looks for
 // such values, and the sequences and heads that have any are done once more, token by token.
@@ -132,11 +134,13 @@ __device__ __forceinline__ float load_tile(float *dst, const T *src, long long t
     }
     return seen;
 }
-// f += A^T B for A [64 k][64 m], B [64 k][64 n] in shared memory; the thread's rows 8 (t / 16).., columns 4 (t % 16)..
-__device__ __forceinline__ void multiply_tn(float (&f)[8][4], const float *A, const float *B) {
+// how far along k there is something in a tile of which n are left, in quads
+__device__ __forceinline__ int quads(int n) { return min(C, (n + 3) & ~3); }
+// f += A^T B for A [K k][64 m], B [K k][64 n] in shared memory; the thread's rows 8 (t / 16).., columns 4 (t % 16)..
+__device__ __forceinline__ void multiply_tn(float (&f)[8][4], const float *A, const float *B, int K) {
     const float *a = A + threadIdx.x / 16 * 8, *b = B + threadIdx.x % 16 * 4;
-#pragma unroll 8
-    for (int k = 0; k < C; k++) {
+#pragma unroll 4
+    for (int k = 0; k < K; k++) {
         const float4 x = *(const float4 *)(a + k * PITCH), y = *(const float4 *)(a + k * PITCH + 4), z = *(const float4 *)(b + k * PITCH);
         const float u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}, v[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
@@ -167,11 +171,11 @@ __device__ __forceinline__ void multiply_nn(float (&f)[8][4], const float *A, co
             }
     }
 }
-// f += A B^T for A [64 m][64 k], B [64 n][64 k]; the thread's rows 8 (t / 16).., columns t % 16 + 16 j, for j up to `last`
-__device__ __forceinline__ void multiply_nt(float (&f)[8][4], const float *A, const float *B, int last) {
+// f += A B^T for A [64 m][K k], B [64 n][K k]; the thread's rows 8 (t / 16).., columns t % 16 + 16 j, for j up to `last`
+__device__ __forceinline__ void multiply_nt(float (&f)[8][4], const float *A, const float *B, int K, int last) {
     const float *a = A + threadIdx.x / 16 * 8 * PITCH, *b = B + threadIdx.x % 16 * PITCH;
 #pragma unroll 2
-    for (int k = 0; k < C; k += 4) {
+    for (int k = 0; k < K; k += 4) {
         float4 u[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) u[i] = *(const float4 *)(a + i * PITCH + k);
@@ -207,7 +211,7 @@ __global__ void __launch_bounds__(TPB) linear_attention_contribution_kernel(Simt
     seen += load_tile<T>(K, k, a.k.token, w.n, d0, a.dk, p.vec[1], by);       // the weights go to the keys
     const int odd = __syncthreads_or(!(seen == 0.0f));
     float f[8][4] = {};
-    multiply_tn(f, K, V);
+    if (d0 + threadIdx.x / 32 * 16 < a.dk) multiply_tn(f, K, V, quads(w.n));      // (a warp has 16 rows)
     float *D = p.ws + (size_t)blockIdx.x * a.dk * a.dv;
     const int c = v0 + threadIdx.x % 16 * 4;
 #pragma unroll
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams
             load_tile<T>(Q, q, a.q.token, w.n, d0, a.dk, p.vec[0]);
             load_tile<T>(K, k, a.k.token, w.n, d0, a.dk, p.vec[1]);
             __syncthreads();
-            multiply_nt(f, Q, K, block);
+            multiply_nt(f, Q, K, quads(a.dk - d0), block);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(TPB) linear_attention_output_kernel(SimtParams
             if (a.dk > C) load_tile<T>(Q, q, a.q.token, w.n, d0, a.dk, p.vec[0]);
             load_tile<float>(K, S + (size_t)d0 * a.dv, a.dv, min(C, a.dk - d0), v0, a.dv, p.vec_state);
             __syncthreads();
-            multiply_nn(f, Q, K, C);
+            multiply_nn(f, Q, K, quads(a.dk - d0));
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
