@@ -28,7 +28,7 @@ class Block:
         self.handle, self.width, self.heads, self.dim, self.dtype = handle, width, heads, head_dim, dtype
         self.inner = heads * head_dim
         self.outs = 4 * self.inner + heads              # q, k, v, gate, and a decay for each head
-        self.w_in, self.w_out = rand(self.outs, width) / width ** 0.5, rand(width, self.inner) / self.inner ** 0.5
+        self.weights = {"in": rand(self.outs, width) / width ** 0.5, "out": rand(width, self.inner) / self.inner ** 0.5}
         self.norm_in, self.norm_heads, self.norm_out, self.norm_next = (1 + 0.1 * rand(n) for n in (width, self.inner, width, width))
         self.scale = 0.5 + 0.1 * rand(width)
         self.plans = {}
@@ -39,18 +39,20 @@ class Block:
             self.plans[key].prepare()
         return self.plans[key]
 
-    def connected(self, x, weight):
+    def connected(self, x, name):
+        weight = self.weights[name]
+
         def make():
             layer = api.Connected(self.handle, x.shape[0], weight.shape[1], weight.shape[0], activation="linear")
             layer.set_weights(weight, torch.zeros(weight.shape[0], device="cuda"))
             return layer
-        return self.plan(("connected", x.shape[0], id(weight)), make).forward(x)
+        return self.plan(("connected", x.shape[0], name), make).forward(x)
 
     def forward(self, x, state, single):
         """x [batch, tokens, width], or [batch, width] for a token of each; `state` is updated."""
         lead, kind = x.shape[:-1], torch.float32 if self.dtype == "f32" else torch.bfloat16
         h, _ = self.handle.norm_gate_residual(x, self.norm_in)
-        y = self.connected(h.reshape(-1, self.width), self.w_in).view(*lead, self.outs)
+        y = self.connected(h.reshape(-1, self.width), "in").view(*lead, self.outs)
         q, k, v, gate = (y[..., i * self.inner:(i + 1) * self.inner].to(kind).view(*lead, self.heads, self.dim) for i in range(4))
         k = k / self.dim ** 0.5
         decay = torch.nn.functional.logsigmoid(y[..., 4 * self.inner:] + 3)
@@ -58,7 +60,7 @@ class Block:
                                                                               self.dim, dtype=self.dtype, scale=self.dim ** -0.5))
         o = layer.step(q, k, v, decay, state) if single else layer.forward(q, k, v, decay, state=state, state_out=state)
         o, _ = self.handle.norm_gate_residual(o.view(-1, self.inner), self.norm_heads, groups=self.heads, gate=gate.reshape(-1, self.inner))
-        o = self.connected(o.float(), self.w_out).view(*lead, self.width)
+        o = self.connected(o.float(), "out").view(*lead, self.width)
         return self.handle.norm_gate_residual(o, self.norm_out, residual=x, channel_scale=self.scale, next_norm="rms", next_weight=self.norm_next)
 
     def state(self, batch):

@@ -18,7 +18,8 @@ constexpr int RECURRENT_TOKENS = 16;        // prompts of up to so many tokens g
 // operations.  A CTA takes `cols` columns of one sequence and head: a thread owns a quad (V = 1: one value) of columns
 // of the rows that are congruent to its own, so that rows are whole lines; all of its part of a state of up to 128 rows is asked
 // for at once, before anything else.  Its parts of q^T S' stay in registers, and are added in the order of the rows.
-// Small CTAs end close together: with one for a whole 128 x 128 state, 64 sequences of 16 heads took 25.4 us (5.3 TB/s).
+// Small CTAs end close together: with one for a whole 128 x 128 state, 64 sequences of 16 heads took 25.4 us (5.3 TB/s), now
+// 24.7 (5.5 TB/s); 333 sequences of 12 heads of 64 x 96 in fp32 36.3 us (5.5 TB/s).
 // The decay is applied as S + expm1(g) S.  exp(g) rounded to fp32 is off by up to 2^-25, the same way at every token of a head with a
 // fixed decay: over a memory of thousands of tokens that adds up to thousands of roundings (a state of 32768 tokens was 3e-4
 // off), while expm1(g) is off by a share of itself.  A decay of zero (expm1 = -1) forgets whatever was there, infinities and NaN too.

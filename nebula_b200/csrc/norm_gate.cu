@@ -137,7 +137,8 @@ __device__ __forceinline__ void group_sums(const NormParams &p, float *parts, fl
 // works on this one's.  A thread has the same columns of every row (launch_rows sees to it where rows are groups of the tensors'), so
 // that addresses are steps of 32 bits; the weights, the block's scales multiplied in, lie in shared memory (in registers they leave
 // room for too few rows in flight: 8192 rows of 4096 took 81 us).  With weights loaded from L1 and addresses worked out for every
-// row, 48 instructions were issued a value: 66 us, and 16384 x 16 x 128 with a gate 72.
+// row, 48 instructions were issued a value: 66 us, and 16384 x 16 x 128 with a gate 72.  Now 55.5 us (4.8 TB/s) and 40.8 us (4.9 TB/s);
+// bound by the issue of instructions, 0.7 a cycle and scheduler, and by HBM.
 template <class T, class R, int V, int NV, bool GATE>
 __global__ void __launch_bounds__(256, 3) norm_gate_rows_kernel(NormParams p) {
     grid_begin();
