@@ -28,7 +28,7 @@ class Block:
         self.handle, self.width, self.heads, self.dim, self.dtype = handle, width, heads, head_dim, dtype
         self.inner = heads * head_dim
         self.outs = 4 * self.inner + heads              # q, k, v, gate, and a decay for each head
-        self.weights = {"in": rand(self.outs, width) / width ** 0.5, "out": rand(width, self.inner) / self.inner ** 0.5}
+        self.w_in, self.w_out = rand(self.outs, width) / width ** 0.5, rand(width, self.inner) / self.inner ** 0.5
         self.norm_in, self.norm_heads, self.norm_out, self.norm_next = (1 + 0.1 * rand(n) for n in (width, self.inner, width, width))
         self.scale = 0.5 + 0.1 * rand(width)
         self.plans = {}
@@ -40,7 +40,7 @@ class Block:
         return self.plans[key]
 
     def connected(self, x, name):
-        weight = self.weights[name]
+        weight = getattr(self, "w_" + name)
 
         def make():
             layer = api.Connected(self.handle, x.shape[0], weight.shape[1], weight.shape[0], activation="linear")
