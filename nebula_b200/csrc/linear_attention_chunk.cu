@@ -18,7 +18,7 @@
 // Bound by HBM where heads are 128 wide and there are as many sequences and heads as SMs: a chunk brings 64 KB and its MMAs are
 // worth 1400 cycles, against 2750 cycles that an SM's share of the bandwidth takes.  What it takes is 3400: the chain of roles that a
 // chunk goes through, and 0.48 instructions a cycle and scheduler.  8 x 4096 tokens, 16 heads of 128: 146 to 152 us (3.6 to 3.7 TB/s);
-// one prompt of 32768 tokens, 8 heads of 128: 117 us; 24 packed prompts of up to 1999 tokens, 12 heads of 64 x 128: 60 us.
+// one prompt of 32768 tokens, 8 heads of 128: 117 to 119 us; 24 packed prompts of up to 1999 tokens, 12 heads of 64 x 128: 60 us.
 //
 // A tensor core multiplies masked entries by zero, which is NaN for infinities and NaN in k and v.  Those are looked for on the
 // way, and a sequence that holds any is done again token by token (recurrence()).
